@@ -1,5 +1,6 @@
 """B200-native token selection (penalties, top-k / top-p / min-p sampling, constraint masks,
-greedy draft acceptance) behind the sampler interface of rizagp/arcinfer.
+greedy draft acceptance) behind the sampler interface of rizagp/arcinfer, and the verification of
+drafted trees over a paged cache (:mod:`arcinfer_b200.kvcache`).
 
 The compute path is the CUDA library ``lib/libarcsample.so`` (sources in ``csrc/``, C ABI in
 ``include/arcsample.h``); this package is the thin Python binding used by the tests and the
@@ -11,6 +12,7 @@ process that only generates inputs does not map the CUDA library.
 from .params import PARAMS_DTYPE, make_params  # noqa: F401
 
 _CAPI_NAMES = ("ArcsError", "accept_batch", "adjusted_batch", "argmax_batch", "dfa_mask", "dflash_select", "lib", "logprobs_batch", "merge_batch", "merge_records", "sample_batch")
+_KVCACHE_NAMES = ("KVCache", "accept_tree", "cache_append", "cache_compact", "cache_fork", "cache_free", "cache_reserve", "tree_attention", "tree_lists")
 
 
 def __getattr__(name):
@@ -19,4 +21,9 @@ def __getattr__(name):
 
         capi = importlib.import_module(".capi", __name__)
         return capi if name == "capi" else getattr(capi, name)
+    if name == "kvcache" or name in _KVCACHE_NAMES:
+        import importlib
+
+        kvcache = importlib.import_module(".kvcache", __name__)
+        return kvcache if name == "kvcache" else getattr(kvcache, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -209,9 +209,66 @@ __global__ void accept_kernel(const int32_t* __restrict__ token, const int32_t* 
   next[s] = nx;
 }
 
+// The walk over a tree: a warp per slot, two nodes a lane, so that a node's children are asked all at
+// once (a vote a step; the first child in index order wins). What bounds it is the latency of one
+// dependent trip for the rows' bounds, one for the nodes and some 40 cycles a step.
+__global__ void __launch_bounds__(128) accept_tree_kernel(const int32_t* __restrict__ token, const int32_t* __restrict__ draft, const int32_t* __restrict__ parent,
+                                                          const int32_t* __restrict__ node_off, int32_t slots, int32_t T, int32_t max_nodes,
+                                                          int32_t* __restrict__ accepted, int32_t* __restrict__ kept, int32_t* __restrict__ next,
+                                                          int32_t* __restrict__ path, int32_t path_stride, int32_t* status) {
+  const int s = (int)(blockIdx.x * 4 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  if (s >= slots) return;
+  const int r0 = node_off[s], r1 = node_off[s + 1];
+  int n = r1 - r0;
+  if (r0 < 0 || r1 < r0 || r1 > T || n > max_nodes) {
+    if (lane == 0) raise_status(status, ARCS_ERR_PAGE);
+    n = 0;
+  }
+  int tk[2], dr[2], pa[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane + 32 * j;
+    const bool in = i < n;
+    tk[j] = in ? token[r0 + i] : -1;
+    dr[j] = in ? draft[r0 + i] : -1;
+    pa[j] = in && i > 0 ? parent[r0 + i] : -1;
+    if (pa[j] >= i) pa[j] = -1;
+  }
+  int mine[2] = {-1, -1}, count = 0, at = 0, last = -1;  // the path's nodes lane, lane + 32
+  while (count < n) {
+    if (lane == (count & 31)) mine[count >> 5] = at;
+    ++count;
+    last = __shfl_sync(0xFFFFFFFFu, at < 32 ? tk[0] : tk[1], at & 31);
+    const unsigned lo = __ballot_sync(0xFFFFFFFFu, pa[0] == at && dr[0] == last);
+    const unsigned hi = __ballot_sync(0xFFFFFFFFu, pa[1] == at && dr[1] == last);
+    if (!(lo | hi)) break;
+    at = lo ? __ffs((int)lo) - 1 : 31 + __ffs((int)hi);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (lane + 32 * j < max_nodes) path[(int64_t)s * path_stride + lane + 32 * j] = mine[j];
+  if (lane == 0) {
+    accepted[s] = count - 1;
+    kept[s] = count;
+    next[s] = last;
+  }
+}
+
 }  // namespace arcs
 
 using namespace arcs;
+
+extern "C" int arcs_accept_tree(const int32_t* token, const int32_t* draft, const int32_t* parent, const int32_t* node_off, int32_t slots, int32_t T,
+                                int32_t max_nodes, int32_t* accepted, int32_t* kept, int32_t* next, int32_t* path, int32_t path_stride, int32_t* status,
+                                void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (!token || !draft || !parent || !node_off || !accepted || !kept || !next || !path || slots <= 0 || T < 0 || max_nodes < 1 || max_nodes > ARCS_TREE_MAX ||
+      path_stride < max_nodes)
+    return set_error(ARCS_ERR_ARG, "accept_tree: bad argument");
+  accept_tree_kernel<<<(unsigned)((slots + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(token, draft, parent, node_off, slots, T, max_nodes, accepted, kept,
+                                                                                                 next, path, path_stride, status);
+  return check_launch("accept_tree");
+}
 
 extern "C" int arcs_accept_batch(const int32_t* token, const int32_t* row_off, const int32_t* draft, const int32_t* draft_off,
                                  int32_t slots, int32_t* accepted, int32_t* next, void* stream) {

@@ -1,0 +1,549 @@
+// The paged cache: room for more tokens, copies that share pages, pages given back, the kept nodes
+// of a verified tree moved together, and the norm and rotation that bring queries and keys there.
+#include "cache.cuh"
+
+namespace arcs {
+
+// ---------------------------------------------------------------- pages taken (reserve, fork)
+// One CTA, because pages go out in order: slot after slot, the lowest free number first. (1) what
+// every slot needs, and the running sum of it; (2) one walk over the pages' counts, 8192 at a time
+// and no further than the last page needed: the r-th free page belongs to the slot whose stretch of
+// the running sum r lies in; (3) the slots' lists. No list of free pages is kept, so none can
+// go stale, and the same pages go out whatever was given back in which order before.
+constexpr int kAllocThreads = 1024;
+
+__device__ __forceinline__ int block_scan_exclusive(int v, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int y = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xFFFFFFFFu, y, o);
+      if (lane >= o) y += z;
+    }
+    warp_sums[lane] = y;
+  }
+  __syncthreads();
+  *total = warp_sums[31];
+  const int before = (w ? warp_sums[w - 1] : 0) + x - v;
+  __syncthreads();
+  return before;
+}
+
+// `ask`: extra[] of reserve, parent[] of fork. done: fork's [slots], 1 where a copy was made.
+template <bool FORK>
+__global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, const int32_t* __restrict__ ask, int32_t* __restrict__ done) {
+  __shared__ int pre[kMaxSlots + 1];   // pages that the slots before this one take
+  __shared__ int base[kMaxSlots];      // where in the slot's list the first new page goes; -1: nothing is done for the slot
+  __shared__ int warp_sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (FORK) pdl_trigger();
+
+  int sum = 0;
+  for (int s0 = 0; s0 < c.slots; s0 += kAllocThreads) {
+    const int s = s0 + tid;
+    int need = 0, at = -1;
+    if (s < c.slots) {
+      const int a = ask[s];
+      if (!FORK && a > 0) {
+        const int used = c.used[s], len = c.len[s];
+        if (used < 0 || used > c.max_pages || len < 0) {
+          raise_status(c.status, ARCS_ERR_PAGE);
+        } else {
+          const int64_t want = ((int64_t)len + a + c.page_size - 1) >> c.page_shift;
+          if (want > c.max_pages) raise_status(c.status, ARCS_ERR_FULL);
+          else if (want > used) { need = (int)want - used; at = used; }
+        }
+      }
+      if (FORK && a >= 0) {
+        bool fine = a < c.slots && a != s && c.used[s] == 0;
+        if (fine) {
+          const int len = c.len[a], used = c.used[a];
+          fine = ask[a] < 0 && len >= 0 && used >= 0 && used <= c.max_pages && (int64_t)len <= ((int64_t)used << c.page_shift);
+          if (fine) { at = len >> c.page_shift; need = (len & (c.page_size - 1)) != 0; }
+        }
+        if (!fine) raise_status(c.status, ARCS_ERR_PAGE);
+      }
+    }
+    if (FORK) {  // (the lists of pages are looked over by a warp each, before anything is promised)
+      for (int q = 0; q < 32; ++q) {
+        const int sq = s0 + warp * 32 + q, atq = __shfl_sync(0xFFFFFFFFu, at, q), needq = __shfl_sync(0xFFFFFFFFu, need, q);
+        if (atq < 0) continue;
+        const int32_t* from = c.table + (int64_t)ask[sq] * c.max_pages;
+        bool fine = true;
+        for (int i = lane; i < atq + needq; i += 32) {
+          const int p = from[i];
+          fine = fine && p >= 0 && p < c.n_pages && c.ref[p] > 0;
+        }
+        if (!__all_sync(0xFFFFFFFFu, fine) && lane == q) {
+          at = -1;
+          need = 0;
+          raise_status(c.status, ARCS_ERR_PAGE);
+        }
+      }
+    }
+    int all;
+    const int before = block_scan_exclusive(need, warp_sums, &all);
+    if (s < c.slots) { pre[s] = sum + before; base[s] = at; }
+    sum += all;
+  }
+  if (tid == 0) pre[c.slots] = sum;
+  __syncthreads();
+
+  int found = 0;  // free pages seen so far
+  for (int p0 = 0; p0 < c.n_pages && found < sum; p0 += kAllocThreads * 8) {
+    unsigned b[8];
+    int mine = 0;
+    const int w0 = p0 + warp * 256;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int p = w0 + j * 32 + lane;
+      b[j] = __ballot_sync(0xFFFFFFFFu, p < c.n_pages && c.ref[p] == 0);
+      mine += __popc(b[j]);
+    }
+    int all;
+    int r0 = found + block_scan_exclusive(lane == 0 ? mine : 0, warp_sums, &all);
+    r0 = __shfl_sync(0xFFFFFFFFu, r0, 0);
+    found += all;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = r0 + __popc(b[j] & ((1u << lane) - 1u));
+      r0 += __popc(b[j]);
+      if (!((b[j] >> lane) & 1u) || r >= sum) continue;
+      int lo = 0, hi = c.slots;  // the last slot with pre[slot] <= r
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      const int p = w0 + j * 32 + lane;
+      c.table[(int64_t)lo * c.max_pages + base[lo] + r - pre[lo]] = p;
+      c.ref[p] = 1;
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && found < sum) raise_status(c.status, ARCS_ERR_FULL);
+
+  // the slots' lists: a warp each
+  for (int s = warp; s < c.slots; s += kAllocThreads / 32) {
+    const int at = base[s], need = pre[s + 1] - pre[s];
+    int32_t* list = c.table + (int64_t)s * c.max_pages;
+    bool ok = at >= 0;
+    if (ok && need > 0 && pre[s + 1] > found) {  // the pages did not suffice: those this slot had been given go back
+      for (int i = lane; i < found - pre[s]; i += 32) {
+        c.ref[list[at + i]] = 0;
+        list[at + i] = -1;
+      }
+      ok = false;
+    }
+    if (FORK) {
+      if (ok) {
+        const int32_t* from = c.table + (int64_t)ask[s] * c.max_pages;
+        for (int i = lane; i < at; i += 32) {
+          const int p = from[i];
+          list[i] = p;
+          atomicAdd(&c.ref[p], 1);
+        }
+        if (lane == 0) {
+          c.used[s] = at + need;
+          c.len[s] = c.len[ask[s]];
+        }
+      }
+      if (lane == 0) done[s] = ok;
+    } else if (ok && lane == 0) {
+      c.used[s] = at + need;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- fork: the rest of the last page
+// A CTA takes one (layer, pool, head) of one copy: `rest` rows of dim values, 16 bytes a thread.
+__global__ void __launch_bounds__(256) fork_copy_kernel(const CacheDev c, const int32_t* __restrict__ parent, const int32_t* __restrict__ done) {
+  pdl_wait();
+  const int s = blockIdx.y;
+  if (!done[s]) return;
+  const int len = c.len[s], rest = len & (c.page_size - 1), last = len >> c.page_shift;
+  if (rest == 0) return;
+  const int from = c.table[(int64_t)parent[s] * c.max_pages + last], to = c.table[(int64_t)s * c.max_pages + last];
+  const int h = blockIdx.x % c.heads, lv = blockIdx.x / c.heads;
+  char* pool = ((lv & 1) ? c.v : c.k) + (lv >> 1) * c.layer_stride + h * c.head_stride;
+  const char* src = pool + from * c.page_stride;
+  char* dst = pool + to * c.page_stride;
+  const int row = c.dim / 8, n = rest * row;  // 16-byte chunks
+  const int shift = 31 - __clz(row);
+  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * 4) {
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * 256;
+      if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + (i >> shift) * c.token_stride + (i & (row - 1)) * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * 256;
+      if (i < n) *reinterpret_cast<uint4*>(dst + (i >> shift) * c.token_stride + (i & (row - 1)) * 16) = x[j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- free
+__device__ __forceinline__ void give_back(const CacheDev& c, int32_t* list, int i) {
+  const int p = list[i];
+  if (p < 0 || p >= c.n_pages) {
+    raise_status(c.status, ARCS_ERR_PAGE);
+  } else if (atomicSub(&c.ref[p], 1) < 1) {  // nobody held it
+    atomicAdd(&c.ref[p], 1);
+    raise_status(c.status, ARCS_ERR_PAGE);
+  }
+  list[i] = -1;
+}
+
+__global__ void __launch_bounds__(256) free_kernel(const CacheDev c, const int32_t* __restrict__ which) {
+  const int s = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (s >= c.slots || which[s] == 0) return;
+  const int used = c.used[s];
+  if (used < 0 || used > c.max_pages) {
+    if (lane == 0) raise_status(c.status, ARCS_ERR_PAGE);
+    return;
+  }
+  for (int i = lane; i < used; i += 32) give_back(c, c.table + (int64_t)s * c.max_pages, i);
+  if (lane == 0) {
+    c.used[s] = 0;
+    c.len[s] = 0;
+  }
+}
+
+// ---------------------------------------------------------------- compact
+// Two launches: the rows move, then the lists change. A slot that the first one refuses is marked in its
+// `used` (a bit that no count has), because what it was refused for, a page with other holders, may
+// look different once the second one gives pages back: every CTA of the first that reads the mark
+// refuses too, and the second takes it off again.
+constexpr int32_t kRefused = 1 << 30;
+
+// Whether a slot's path can be followed; asked by a whole warp, the same answer in every lane.
+template <bool HOLDERS>
+__device__ __forceinline__ bool path_fine(const CacheDev& c, int s, int used, int kept, const int32_t* __restrict__ path, int path_stride) {
+  const int lane = threadIdx.x & 31, len = c.len[s];
+  bool fine = kept <= ARCS_TREE_MAX && kept <= path_stride && len >= 0 && used >= 0 && used <= c.max_pages && (int64_t)len <= ((int64_t)used << c.page_shift);
+  if (fine) {
+    for (int i = lane; i < kept; i += 32) {
+      const int node = path[i], before = i ? path[i - 1] : -1;
+      if (node <= before || node >= ARCS_TREE_MAX || (int64_t)len + node >= ((int64_t)used << c.page_shift)) {
+        fine = false;
+        continue;
+      }
+      const int from = c.table[(int64_t)s * c.max_pages + ((len + node) >> c.page_shift)];
+      // (the list holds ascending nodes, so node >= i and this place lies inside the slot's pages, too; the
+      // first test decides before a list that is not ascending could lead elsewhere)
+      fine = fine && from >= 0 && from < c.n_pages;
+      if (node < i) { fine = false; continue; }
+      if (node > i) {
+        const int to = c.table[(int64_t)s * c.max_pages + ((len + i) >> c.page_shift)];
+        fine = fine && to >= 0 && to < c.n_pages && (!HOLDERS || c.ref[to] == 1);
+      }
+    }
+  }
+  return __all_sync(0xFFFFFFFFu, fine);
+}
+
+// Rows move towards the front only (node >= its place), and a thread keeps to one 16-byte column of
+// one (layer, pool, head): it reads up to eight rows before it writes them, in ascending order, so no
+// row is written before it has been read.
+__global__ void __launch_bounds__(256) compact_move_kernel(const CacheDev c, const int32_t* __restrict__ kept_, const int32_t* __restrict__ path_, int path_stride) {
+  pdl_trigger();
+  __shared__ int64_t from[ARCS_TREE_MAX], to[ARCS_TREE_MAX];
+  __shared__ int s_first;
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const int kept = kept_[s];
+  if (kept <= 0) return;
+  const int32_t* path = path_ + (int64_t)s * path_stride;
+  if (tid < 32) {
+    const int used = *(volatile int32_t*)(c.used + s);
+    const bool fine = path_fine<true>(c, s, used, kept, path, path_stride);
+    if (!fine && blockIdx.x == 0 && tid == 0 && used >= 0 && used <= c.max_pages) c.used[s] = used | kRefused;
+    int first = kept;  // nodes before it stay where they are
+    if (fine) {
+      const int len = c.len[s];
+      for (int i = tid; i < kept; i += 32) {
+        const int a = len + path[i], b = len + i;
+        if (a != b) first = min(first, i);
+        from[i] = c.table[(int64_t)s * c.max_pages + (a >> c.page_shift)] * c.page_stride + (a & (c.page_size - 1)) * c.token_stride;
+        to[i] = c.table[(int64_t)s * c.max_pages + (b >> c.page_shift)] * c.page_stride + (b & (c.page_size - 1)) * c.token_stride;
+      }
+    }
+    first = __reduce_min_sync(0xFFFFFFFFu, first);
+    if (tid == 0) s_first = first;
+  }
+  __syncthreads();
+  const int first = s_first;
+  if (first >= kept) return;
+  const int row = c.dim / 8, cols = c.layers * 2 * c.heads * row;
+  const int col = blockIdx.x * 256 + tid;
+  if (col >= cols) return;
+  const int d = col % row, h = col / row % c.heads, lv = col / row / c.heads;
+  char* pool = ((lv & 1) ? c.v : c.k) + (lv >> 1) * c.layer_stride + h * c.head_stride + d * 16;
+  for (int i0 = first; i0 < kept; i0 += 8) {
+    uint4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j < kept) x[j] = *reinterpret_cast<const uint4*>(pool + from[i0 + j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j < kept) *reinterpret_cast<uint4*>(pool + to[i0 + j]) = x[j];
+  }
+}
+
+__global__ void __launch_bounds__(256) compact_lists_kernel(const CacheDev c, const int32_t* __restrict__ kept_, const int32_t* __restrict__ path_, int path_stride,
+                                                            int32_t* len_out) {
+  pdl_wait();
+  const int s = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (s >= c.slots) return;
+  const int kept = max(0, kept_[s]), len = c.len[s], used = c.used[s];
+  const bool fine = path_fine<false>(c, s, used, kept, path_ + (int64_t)s * path_stride, path_stride);
+  __syncwarp();
+  if (!fine) {
+    if (lane == 0) {
+      if (used >= kRefused && used <= kRefused + c.max_pages) c.used[s] = used - kRefused;
+      raise_status(c.status, ARCS_ERR_PAGE);
+      len_out[s] = len;
+    }
+    return;
+  }
+  const int left = (len + kept + c.page_size - 1) >> c.page_shift;
+  for (int i = left + lane; i < used; i += 32) give_back(c, c.table + (int64_t)s * c.max_pages, i);
+  __syncwarp();
+  if (lane == 0) {
+    if (left < used) c.used[s] = left;
+    len_out[s] = len + kept;
+  }
+}
+
+// ---------------------------------------------------------------- append
+struct AppendDev {
+  CacheDev c;  // k and v: the layer's
+  const char* q;
+  const char* k;
+  const char* v;
+  char* q_out;
+  int64_t q_stride, k_stride, v_stride, q_out_stride;  // bytes
+  const float* q_weight;
+  const float* k_weight;
+  float eps;
+  int32_t T, Hq, rot, interleaved;
+  const double* inv_freq;
+  const int32_t* pos;
+  const int32_t* node_off;
+};
+
+template <typename T> struct Half2Of;
+template <> struct Half2Of<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 widen(uint32_t w) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Half2Of<__half> {
+  static __device__ __forceinline__ float2 widen(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// One CTA a row. The turns of the rotation are found once (in fp64: pos * inv_freq / 2 pi less its
+// whole part, so a position of any size leaves an angle exact to fp32) and shared by all heads; a
+// head is DIM / 8 neighbouring lanes with 16 bytes each.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
+  __shared__ float2 turn[DIM / 2];
+  __shared__ int s_slot;
+  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes;
+  const int t = blockIdx.x, tid = threadIdx.x;
+  if (tid < 32) {
+    const int s = slot_of_row(a.node_off, a.c.slots, t);
+    if (tid == 0) s_slot = s;
+  }
+  if (tid >= 128 && tid - 128 < a.rot / 2) {
+    const int i = tid - 128;
+    const double turns = (double)a.pos[t] * a.inv_freq[i] * 0.15915494309189533577;
+    float sn, cs;
+    sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
+    turn[i] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  const int s = s_slot;
+  if (s < 0) return;  // behind the last slot's rows
+  const int64_t place = (int64_t)a.c.len[s] + (t - a.node_off[s]), list = place >> a.c.page_shift;
+  int page = -1;
+  if (place >= 0 && list < a.c.used[s] && list < a.c.max_pages) page = a.c.table[(int64_t)s * a.c.max_pages + list];
+  if (page < 0 || page >= a.c.n_pages) {
+    page = -1;
+    if (tid == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
+  }
+  const int64_t at = page * a.c.page_stride + (place & (a.c.page_size - 1)) * a.c.token_stride;
+  const int lane = tid % kLanes, e0 = lane * 8;
+  const int all = a.Hq + 2 * a.c.heads;
+  for (int g0 = 0; g0 < all; g0 += kGroups) {
+    const int g = g0 + tid / kLanes;
+    const bool live = g < all;
+    const bool is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
+    const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
+    const char* src = is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (live) x = *reinterpret_cast<const uint4*>(src + (int64_t)h * (DIM * 2) + lane * 16);
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = Half2Of<T>::widen(j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w);
+      y[2 * j] = f.x;
+      y[2 * j + 1] = f.y;
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+    const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+    if (w && live) {
+      const float r = 1.0f / sqrtf(ss * (1.0f / DIM) + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * r * __ldg(w + e0 + j);
+    }
+    const int half = a.rot / 2;
+    if (a.interleaved) {
+      if (!is_v && e0 < a.rot) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float2 f = turn[(e0 + j) / 2];
+          const float u = y[j] * f.x - y[j + 1] * f.y;
+          y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
+          y[j] = u;
+        }
+      }
+    } else if (a.rot) {
+      // the pair's other value is in the lane rot / 16 further, or before
+      const bool first = e0 < half;
+      const int other = first ? lane + half / 8 : e0 < a.rot ? lane - half / 8 : lane;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
+        if (!is_v && e0 < a.rot) {
+          const float2 f = turn[(first ? e0 : e0 - half) + j];
+          y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
+        }
+      }
+    }
+    if (!live || (!is_q && page < 0)) continue;
+    if (!is_v) x = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
+    char* dst = is_q ? a.q_out + t * a.q_out_stride + (int64_t)h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
+    *reinterpret_cast<uint4*>(dst + lane * 16) = x;
+  }
+}
+
+}  // namespace arcs
+
+using namespace arcs;
+
+extern "C" int arcs_cache_reserve(const arcs_cache* cache, const int32_t* extra, void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (const char* f = cache_fault(cache, true)) return bad_argument("cache_reserve", f);
+  if (!extra) return bad_argument("cache_reserve", "no list of extra tokens");
+  alloc_kernel<false><<<1, kAllocThreads, 0, static_cast<cudaStream_t>(stream)>>>(cache_dev(cache), extra, nullptr);
+  return check_launch("cache_reserve");
+}
+
+extern "C" int arcs_cache_fork(const arcs_cache* cache, const int32_t* parent, int32_t* done, void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (const char* f = cache_fault(cache, true)) return bad_argument("cache_fork", f);
+  if (!parent || !done) return bad_argument("cache_fork", "no list of parents, or none for what was done");
+  const CacheDev c = cache_dev(cache);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  alloc_kernel<true><<<1, kAllocThreads, 0, st>>>(c, parent, done);
+  if (int rc = check_launch("cache_fork")) return rc;
+  const dim3 grid((unsigned)(c.layers * 2 * c.heads), (unsigned)c.slots);
+  launch_behind(fork_copy_kernel, grid, dim3(256), 0, st, c, parent, done);
+  return check_launch("cache_fork");
+}
+
+extern "C" int arcs_cache_free(const arcs_cache* cache, const int32_t* which, void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (const char* f = cache_fault(cache, true)) return bad_argument("cache_free", f);
+  if (!which) return bad_argument("cache_free", "no list of slots");
+  free_kernel<<<(unsigned)((cache->slots + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(cache_dev(cache), which);
+  return check_launch("cache_free");
+}
+
+extern "C" int arcs_cache_compact(const arcs_cache* cache, const int32_t* kept, const int32_t* path, int32_t path_stride, int32_t* len_out, void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (const char* f = cache_fault(cache, true)) return bad_argument("cache_compact", f);
+  if (!kept || !path || !len_out || path_stride < 1) return bad_argument("cache_compact", "no paths, or nowhere to write the lengths");
+  const CacheDev c = cache_dev(cache);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t cols = (int64_t)c.layers * 2 * c.heads * (c.dim / 8);
+  if (cols > 0x7FFFFF00ll) return bad_argument("cache_compact", "layers x heads x dim is too large");
+  compact_move_kernel<<<dim3((unsigned)((cols + 255) / 256), (unsigned)c.slots), 256, 0, st>>>(c, kept, path, path_stride);
+  if (int rc = check_launch("cache_compact")) return rc;
+  launch_behind(compact_lists_kernel, dim3((unsigned)((c.slots + 7) / 8)), dim3(256), 0, st, c, kept, path, path_stride, len_out);
+  return check_launch("cache_compact");
+}
+
+extern "C" int arcs_cache_append(const arcs_append_args* g, void* stream) {
+  if (int inj = fault_injected()) return inj;
+  if (!g) return bad_argument("cache_append", "no arguments");
+  if (const char* f = cache_fault(g->cache, false)) return bad_argument("cache_append", f);
+  const arcs_cache* c = g->cache;
+  if (g->layer < 0 || g->layer >= c->layers) return bad_argument("cache_append", "no such layer");
+  if (g->T < 0 || g->Hq < 1 || g->Hq > 65536) return bad_argument("cache_append", "T or Hq out of range");
+  if (g->T == 0) return ARCS_OK;
+  if (!g->q || !g->k || !g->v || !g->q_out || !g->pos || !g->node_off || (g->rot > 0 && !g->inv_freq)) return bad_argument("cache_append", "a null pointer");
+  if (g->rot < 0 || g->rot > c->dim || g->rot % 16) return bad_argument("cache_append", "rot is not a multiple of 16 up to dim");
+  const int64_t qrow = (int64_t)g->Hq * c->dim, krow = (int64_t)c->heads * c->dim;
+  if (((g->q_stride | g->k_stride | g->v_stride | g->q_out_stride) & 7) || g->q_stride < qrow || g->q_out_stride < qrow || g->k_stride < krow || g->v_stride < krow)
+    return bad_argument("cache_append", "a stride is not a multiple of 8 elements, or shorter than a row");
+  if ((reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->k) | reinterpret_cast<uintptr_t>(g->v) | reinterpret_cast<uintptr_t>(g->q_out)) & 15)
+    return bad_argument("cache_append", "a tensor is not 16-byte aligned");
+  if (!(g->eps >= 0.0f)) return bad_argument("cache_append", "eps is negative");
+  AppendDev a;
+  a.c = cache_dev(c);
+  a.c.k += g->layer * a.c.layer_stride;
+  a.c.v += g->layer * a.c.layer_stride;
+  a.q = static_cast<const char*>(g->q);
+  a.k = static_cast<const char*>(g->k);
+  a.v = static_cast<const char*>(g->v);
+  a.q_out = static_cast<char*>(g->q_out);
+  a.q_stride = g->q_stride * 2;
+  a.k_stride = g->k_stride * 2;
+  a.v_stride = g->v_stride * 2;
+  a.q_out_stride = g->q_out_stride * 2;
+  a.q_weight = g->q_weight;
+  a.k_weight = g->k_weight;
+  a.eps = g->eps;
+  a.T = g->T;
+  a.Hq = g->Hq;
+  a.rot = g->rot;
+  a.interleaved = g->interleaved;
+  a.inv_freq = g->inv_freq;
+  a.pos = g->pos;
+  a.node_off = g->node_off;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)g->T;
+#define ARCS_LAUNCH(TYPE)                                                     \
+  do {                                                                        \
+    if (c->dim == 64) append_kernel<TYPE, 64><<<grid, 256, 0, st>>>(a);       \
+    else if (c->dim == 128) append_kernel<TYPE, 128><<<grid, 256, 0, st>>>(a); \
+    else append_kernel<TYPE, 256><<<grid, 256, 0, st>>>(a);                   \
+  } while (0)
+  if (c->dtype == ARCS_BF16) ARCS_LAUNCH(__nv_bfloat16);
+  else ARCS_LAUNCH(__half);
+#undef ARCS_LAUNCH
+  return check_launch("cache_append");
+}

@@ -36,10 +36,12 @@ typedef enum {
   ARCS_ERR_LIST = 5,       /* a row's history / bias list is longer than max_hist / max_bias */
   ARCS_ERR_TIMEOUT = 6,    /* device side: a bounded wait ran out (status word only) */
   ARCS_ERR_INJECTED = 7,   /* host-side fault injection (ARCS_FAIL_CALL=N environment variable) */
-  ARCS_ERR_UNSUPPORTED = 8 /* jcon: the schema (or this step's table) is outside what the automaton expresses */
+  ARCS_ERR_UNSUPPORTED = 8,/* jcon: the schema (or this step's table) is outside what the automaton expresses */
+  ARCS_ERR_PAGE = 9,       /* device side: a slot's lists name a page, a place or a node that is not there (status word only) */
+  ARCS_ERR_FULL = 10       /* device side: no free pages left for a slot, or its list of pages is full (status word only) */
 } arcs_status;
 
-typedef enum { ARCS_F32 = 0, ARCS_BF16 = 1 } arcs_dtype;
+typedef enum { ARCS_F32 = 0, ARCS_BF16 = 1, ARCS_F16 = 2 /* the cache's calls only */ } arcs_dtype;
 
 /* One row's sampling parameters: SamplingParams (tools/sampler.h:15-26) field for field,
  * without the seed (the uniform draw u is an explicit input) and without the logit_bias
@@ -384,6 +386,132 @@ typedef struct {
 
 size_t arcs_dflash_workspace_bytes(int32_t slots, int32_t nd, int32_t V, int32_t topk);
 int arcs_dflash_select(const arcs_dflash_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The paged cache, and the verification of a TREE of drafts over it (no counterpart in the
+ * reference, which verifies a chain of drafts over one contiguous cache per slot).
+ * A step of a server: arcs_cache_reserve (room for every slot's nodes), per layer arcs_cache_append
+ * (norm, rotation, keys and values to their pages) and arcs_tree_attention, then the head's logits,
+ * arcs_argmax_batch or arcs_sample_batch over all nodes, arcs_accept_tree, arcs_cache_compact.
+ *
+ * A slot is a sequence; its nodes in a step are the rows node_off[s] .. node_off[s+1] - 1 of the
+ * step's tensors (an empty range: a slot without work; rows past node_off[slots] are left alone).
+ * Node 0 is the root, the last token that is certain; a node's parent comes before it. Node j's key
+ * and value lie at place len[s] + j of the slot, behind the len[s] tokens that are settled.
+ * Place p of slot s is row p % page_size of page table[s * max_pages + p / page_size].
+ * All calls are dense over the slots, so no slot can be named twice.
+ * ---------------------------------------------------------------------------------------- */
+#define ARCS_TREE_MAX 64       /* most nodes of a slot's tree */
+typedef struct {
+  /* element (layer l, page p, head h, row t, value d) of a pool lies at l * layer_stride + p * page_stride +
+   * h * head_stride + t * token_stride + d; strides in elements, multiples of 8, and rows do not overlap */
+  void* k;                     /* the two pools (device), 16-byte aligned, laid out alike */
+  void* v;
+  int32_t dtype;               /* ARCS_BF16 or ARCS_F16 */
+  int32_t layers, n_pages;
+  int32_t page_size;           /* 16, 32, 64, 128 or 256 tokens */
+  int32_t heads, dim;          /* key heads; dim 64, 128 or 256 */
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+  int32_t slots, max_pages;    /* slots <= 4096 */
+  int32_t* table;              /* [slots][max_pages] */
+  int32_t* used;               /* [slots] pages a slot holds: the first used[s] entries of its row */
+  int32_t* ref;                /* [n_pages] slots that hold a page; 0: free */
+  int32_t* len;                /* [slots] settled tokens */
+  int32_t* status;             /* optional device word: 0 or an arcs_status set by the kernels */
+} arcs_cache;
+
+/* Room for extra[s] more tokens behind len[s] (extra[s] <= 0: nothing): pages are taken from the free
+ * ones, the lowest number first, slot after slot. When they run out, or a slot's list would pass
+ * max_pages, ARCS_ERR_FULL is raised: a slot whose list would pass max_pages gets none, and from the
+ * first slot on for which the pages do not suffice no slot gets any. */
+int arcs_cache_reserve(const arcs_cache* cache, const int32_t* extra, void* stream);
+/* slot s becomes a copy of slot parent[s] (parent[s] < 0: nothing): full pages are shared, the rest of
+ * the last one is copied, in all layers, to a page of its own (chosen as in arcs_cache_reserve;
+ * ARCS_ERR_FULL alike). Slot s must hold no pages and parent[s] must not itself become a copy in this
+ * call (ARCS_ERR_PAGE, and the slot is left as it is). Afterwards both may grow on their own.
+ * done[s]: 1 where a copy was made, else 0. */
+int arcs_cache_fork(const arcs_cache* cache, const int32_t* parent, int32_t* done, void* stream);
+/* the pages of every slot with which[s] != 0 are given back (a shared one stays with its other
+ * holders): len[s] = used[s] = 0, its list -1. */
+int arcs_cache_free(const arcs_cache* cache, const int32_t* which, void* stream);
+/* After a verification: the kept[s] nodes path[s * path_stride + i] (strictly ascending, the order of
+ * arcs_accept_tree) become the slot's next tokens: in all layers, node path[i]'s key and value move to
+ * place len[s] + i; len_out[s] = len[s] + kept[s] (len_out may be cache->len); pages past the last of
+ * these tokens are given back. kept[s] = 0: only that last part. A slot whose path is not ascending,
+ * passes ARCS_TREE_MAX nodes or leaves the slot's pages is left as it is (len_out[s] = len[s]) and
+ * ARCS_ERR_PAGE is raised; also where a page that would be written has other holders. */
+int arcs_cache_compact(const arcs_cache* cache, const int32_t* kept, const int32_t* path, int32_t path_stride, int32_t* len_out,
+                       void* stream);
+
+/* Norm and rotation of the step's queries and keys, head by head, and the way of keys and values into
+ * one layer of the cache, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight          (weight NULL: y = x)
+ *   (a, b) -> (a cos - b sin, a sin + b cos), angle pos[t] * inv_freq[i], for the pairs i < rot / 2 of
+ *   the first rot values: (y[i], y[i + rot/2]), or (y[2i], y[2i+1]) with interleaved != 0.
+ * Sums, norm and rotation are in 32 bits, rounded once at the end; the angle's turns are counted in 64
+ * bits, so that far positions lose nothing. Any number of nodes per slot (prompts too). A node whose
+ * place lies outside the slot's pages raises ARCS_ERR_PAGE; its key and value are not written. Pages
+ * that are written should have no other holder (arcs_cache_fork sees to that). */
+typedef struct {
+  const arcs_cache* cache;     /* (host) */
+  int32_t layer;
+  int32_t T, Hq;               /* rows of the tensors below, query heads */
+  const void* q;               /* [T][Hq][dim] of the cache's dtype, rows q_stride elements apart, heads contiguous */
+  const void* k;               /* [T][heads][dim] */
+  const void* v;               /* [T][heads][dim] */
+  int64_t q_stride, k_stride, v_stride;   /* multiples of 8; the tensors 16-byte aligned */
+  void* q_out;                 /* [T][Hq][dim], rows q_out_stride apart; may be q itself */
+  int64_t q_out_stride;
+  const float* q_weight;       /* [dim], or NULL: queries are not normalised */
+  const float* k_weight;       /* [dim], or NULL: keys are not normalised */
+  float eps;
+  int32_t rot;                 /* values rotated: 0 .. dim, a multiple of 16 */
+  int32_t interleaved;
+  const double* inv_freq;      /* [rot / 2] */
+  const int32_t* pos;          /* [T] positions (of a tree: len + depth) */
+  const int32_t* node_off;     /* [slots + 1] */
+} arcs_append_args;
+int arcs_cache_append(const arcs_append_args* args, void* stream);
+
+/* Attention of every slot's nodes over its settled tokens and those nodes that their masks name:
+ *   out = sum_p softmax(scale * q . k_p) v_p,   lse = log sum_p exp(scale * q . k_p)
+ * over all p < len[s] and p = len[s] + j for the bits j of mask[t] (nodes that the slot does not have
+ * are ignored; a node's own bit is taken as it stands, too). mask NULL: a chain, node i sees the nodes
+ * 0 .. i. Query head h reads key head h / (Hq / heads). A row that sees nothing gets zeros and lse
+ * -inf. What lies in masked places, and behind the last node, has no influence, NaN included.
+ * Scores, statistics and sums are held in 32 bits; the weights are rounded to the cache's dtype before
+ * the product with the values. A slot whose lists do not hold its tokens, or with more than max_nodes
+ * nodes, raises ARCS_ERR_PAGE and its rows hold no result. */
+typedef struct {
+  const arcs_cache* cache;     /* (host); `ref` is not used */
+  int32_t layer;
+  int32_t T, Hq;               /* rows of q and out, query heads: a multiple of cache->heads, at most 64 times it */
+  const void* q;               /* of the cache's dtype, 16-byte aligned */
+  int64_t q_token_stride, q_head_stride;      /* elements, multiples of 8 */
+  void* out;                   /* as q */
+  int64_t out_token_stride, out_head_stride;
+  float* lse;                  /* [T][Hq] optional, contiguous */
+  const int32_t* node_off;     /* [slots + 1] */
+  const uint64_t* mask;        /* [T] or NULL */
+  int32_t max_nodes;           /* 1 .. ARCS_TREE_MAX: no slot has more */
+  float scale;                 /* > 0 */
+  void* workspace;             /* arcs_tree_attention_workspace_bytes(), 16-byte aligned; needs no initialisation; one for each call that may overlap another */
+  size_t workspace_bytes;
+} arcs_tree_attention_args;
+size_t arcs_tree_attention_workspace_bytes(int32_t slots, int32_t heads, int32_t Hq, int32_t dim, int32_t max_nodes);
+int arcs_tree_attention(const arcs_tree_attention_args* args, void* stream);
+
+/* accept_tree: arcs_accept_batch's walk over trees. token[t]: the token chosen at node t; draft[t]: the
+ * token that node t stands for; parent[t]: its parent's index within the slot (the root's is not read;
+ * a node whose parent does not come before it is never reached). From the root on: the first child
+ * whose draft equals the token chosen at the node, until there is none. accepted[s] = drafts on the
+ * path (-1 for a slot without nodes), next[s] = the token chosen at its end (-1), path[s * path_stride
+ * + i] = its nodes, the root first, then -1 up to max_nodes; kept[s] = nodes on it (accepted[s] + 1):
+ * what arcs_cache_compact takes. A slot with more than max_nodes nodes, or rows outside 0 .. T - 1, is
+ * taken as one without, and raises ARCS_ERR_PAGE in `status` (optional). */
+int arcs_accept_tree(const int32_t* token, const int32_t* draft, const int32_t* parent, const int32_t* node_off, int32_t slots, int32_t T,
+                     int32_t max_nodes, int32_t* accepted, int32_t* kept, int32_t* next, int32_t* path, int32_t path_stride, int32_t* status,
+                     void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Host-buffer entry points: what a host application that keeps its logits in host memory
