@@ -1,22 +1,10 @@
 // Attention of the nodes of drafted trees over a paged cache.
-#include "cache.cuh"
+#include "tree_tiles.cuh"
 
 namespace arcs {
 
-struct TreeDev {
-  CacheDev c;  // k and v: the layer's
-  const char* q;
-  char* out;
-  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
-  float* lse;
-  const int32_t* node_off;
-  const unsigned long long* mask;
-  int32_t T, Hq, group, max_nodes;
-  float scale_log2;  // scale * log2 e
-};
-
-// One warp a row (a node and a query head): a running maximum and sum over the places it sees, the
-// values added up as they come.
+// For pools whose rows no tensor map can name (strides that are not multiples of one another): one warp a
+// row, a running maximum and sum over the places it sees, the values added up as they come.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(128) tree_rows_kernel(const TreeDev a) {
   constexpr int kPer = DIM / 32;
@@ -77,11 +65,73 @@ __global__ void __launch_bounds__(128) tree_rows_kernel(const TreeDev a) {
 
 }  // namespace arcs
 
+namespace {
+
 using namespace arcs;
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// How a pool's rows lie: as rows `token` apart that pages and heads are whole numbers of, or, with a
+// token's heads side by side, as such rows of heads. false: neither.
+struct RowPlan {
+  bool by_row;
+  int64_t page_rows, head_rows, rows;
+};
+bool plan_rows(const arcs_cache* c, RowPlan* r) {
+  const int64_t ts = c->token_stride, ps = c->n_pages > 1 ? c->page_stride : 0, hs = c->heads > 1 ? c->head_stride : 0;
+  if (ps % ts) return false;
+  r->page_rows = ps / ts;
+  r->by_row = hs % ts == 0;
+  r->head_rows = r->by_row ? hs / ts : 0;
+  if (!r->by_row && (ts % hs || hs * c->heads > ts)) return false;
+  r->rows = (c->n_pages - 1) * r->page_rows + (c->heads - 1) * r->head_rows + c->page_size;
+  return r->rows < 0x7FFFFF00ll && ts * 2 < (1ll << 40);
+}
+
+bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const RowPlan& r, int keys) {
+  const int box = c->page_size < keys ? c->page_size : keys;
+  const int64_t hs = c->heads > 1 ? c->head_stride : c->dim;
+  const cuuint64_t dims[3] = {(cuuint64_t)c->dim, (cuuint64_t)(r.by_row ? r.rows : c->heads), (cuuint64_t)(r.by_row ? 1 : r.rows)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(r.by_row ? c->token_stride : hs) * 2, (cuuint64_t)c->token_stride * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)(r.by_row ? box : 1), (cuuint32_t)(r.by_row ? 1 : box)}, steps[3] = {1, 1, 1};
+  return encode_tiled()(map, c->dtype == ARCS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kCtas = kSmCount;
+int mode_of(int dim, int rows) { return dim == 256 ? kSingle : rows > 128 ? kPair : kSplit; }
+int rows_of(int mode) { return mode == kPair ? 256 : 128; }
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+template <typename T, int DIM, int MODE>
+int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a, cudaStream_t st) {
+  using P = TilePlan<DIM, MODE>;
+  static std::atomic<unsigned long long> attr_done{0};
+  const cudaError_t e = ensure_dynamic_smem(tree_tiles_kernel<T, DIM, MODE>, P::kSmem, attr_done);
+  if (e != cudaSuccess) return set_error(ARCS_ERR_CUDA, cudaGetErrorString(e));
+  tree_tiles_kernel<T, DIM, MODE><<<kCtas, P::kThreadsT, P::kSmem, st>>>(mk, mv, a);
+  if (int rc = check_launch("tree_attention")) return rc;
+  launch_behind(join_kernel<T, DIM, MODE>, dim3((unsigned)(((int64_t)a.T * a.Hq + 7) / 8)), dim3(256), 0, st, a, kCtas);
+  return check_launch("tree_attention");
+}
+
+}  // namespace
+
 extern "C" size_t arcs_tree_attention_workspace_bytes(int32_t slots, int32_t heads, int32_t Hq, int32_t dim, int32_t max_nodes) {
-  if (slots < 1 || heads < 1 || Hq < heads || Hq % heads || (dim != 64 && dim != 128 && dim != 256) || max_nodes < 1 || max_nodes > ARCS_TREE_MAX) return 0;
-  return 256;
+  if (slots < 1 || heads < 1 || Hq < heads || Hq % heads || Hq / heads > 64 || (dim != 64 && dim != 128 && dim != 256) || max_nodes < 1 || max_nodes > ARCS_TREE_MAX) return 0;
+  const int rows = max_nodes * (Hq / heads), most = rows_of(mode_of(dim, rows));
+  const size_t blocks = (size_t)kCtas * 2 * (rows < most ? rows : most);
+  return round16(((size_t)slots + 1) * 4) + round16(blocks * 8) + blocks * dim * 4;
 }
 
 extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stream) {
@@ -99,8 +149,9 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
       g->out_token_stride < c->dim || g->out_head_stride < c->dim)
     return bad_argument("tree_attention", "a stride is not a multiple of 8 elements, or below dim");
   if ((reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->out)) & 15) return bad_argument("tree_attention", "a tensor is not 16-byte aligned");
-  if (!g->workspace || g->workspace_bytes < arcs_tree_attention_workspace_bytes(c->slots, c->heads, g->Hq, c->dim, g->max_nodes))
-    return set_error(ARCS_ERR_WORKSPACE, "tree_attention: workspace too small");
+  if (!g->workspace || g->workspace_bytes < arcs_tree_attention_workspace_bytes(c->slots, c->heads, g->Hq, c->dim, g->max_nodes) ||
+      (reinterpret_cast<uintptr_t>(g->workspace) & 15))
+    return set_error(ARCS_ERR_WORKSPACE, "tree_attention: workspace too small, or not 16-byte aligned");
   TreeDev a;
   a.c = cache_dev(c);
   a.c.k += g->layer * a.c.layer_stride;
@@ -120,9 +171,40 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
   a.max_nodes = g->max_nodes;
   a.scale_log2 = g->scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t rows = (int64_t)g->T * g->Hq;
-  if (rows > 0x1FFFFFFF0ll) return bad_argument("tree_attention", "too many rows");
-  const unsigned grid = (unsigned)((rows + 3) / 4);
+  const int64_t all_rows = (int64_t)g->T * g->Hq;
+  if (all_rows > 0x1FFFFFFF0ll) return bad_argument("tree_attention", "too many rows");
+
+  RowPlan r;
+  if (plan_rows(c, &r)) {
+    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = c->dim == 256 ? 64 : 128;
+    if ((((int64_t)c->max_pages * c->page_size + keys - 1) / keys) * c->slots * c->heads * ((rows + most - 1) / most) > 0x7FFFFFFFll)
+      return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
+    if (!encode_tiled()) return set_error(ARCS_ERR_CUDA, "tree_attention: the driver makes no tensor maps");
+    CUtensorMap mk, mv;
+    if (!make_map(&mk, c, a.c.k, r, keys) || !make_map(&mv, c, a.c.v, r, keys)) return set_error(ARCS_ERR_CUDA, "tree_attention: no tensor map for these pools");
+    a.by_row = r.by_row;
+    a.page_rows = (int32_t)r.page_rows;
+    a.head_rows = (int32_t)r.head_rows;
+    a.no_row = (int32_t)r.rows;
+    a.part_rows = rows < most ? rows : most;
+    char* ws = static_cast<char*>(g->workspace);
+    const size_t blocks = (size_t)kCtas * 2 * a.part_rows;
+    a.prefix = reinterpret_cast<uint32_t*>(ws);
+    a.part_stat = reinterpret_cast<float2*>(ws + round16(((size_t)c->slots + 1) * 4));
+    a.part = reinterpret_cast<float*>(ws + round16(((size_t)c->slots + 1) * 4) + round16(blocks * 8));
+#define ARCS_LAUNCH(TYPE)                                                                \
+  do {                                                                                   \
+    if (c->dim == 256) return launch_tiles<TYPE, 256, kSingle>(mk, mv, a, st);           \
+    if (c->dim == 128 && mode == kPair) return launch_tiles<TYPE, 128, kPair>(mk, mv, a, st); \
+    if (c->dim == 128) return launch_tiles<TYPE, 128, kSplit>(mk, mv, a, st);            \
+    if (mode == kPair) return launch_tiles<TYPE, 64, kPair>(mk, mv, a, st);              \
+    return launch_tiles<TYPE, 64, kSplit>(mk, mv, a, st);                                \
+  } while (0)
+    if (c->dtype == ARCS_BF16) ARCS_LAUNCH(__nv_bfloat16);
+    else ARCS_LAUNCH(__half);
+#undef ARCS_LAUNCH
+  }
+  const unsigned grid = (unsigned)((all_rows + 3) / 4);
 #define ARCS_LAUNCH(TYPE)                                                       \
   do {                                                                          \
     if (c->dim == 64) tree_rows_kernel<TYPE, 64><<<grid, 128, 0, st>>>(a);      \

@@ -1,0 +1,710 @@
+// Tree attention on the tensor cores: tiles of 128 rows (a node and a query head each) against tiles of
+// keys and values that come from their pages by tiled copies.
+#pragma once
+#include "cache.cuh"
+#include "tcgen05.cuh"
+
+namespace arcs {
+
+struct TreeDev {
+  CacheDev c;  // k and v: the layer's
+  const char* q;
+  char* out;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
+  float* lse;
+  const int32_t* node_off;
+  const unsigned long long* mask;
+  int32_t T, Hq, group, max_nodes;
+  float scale_log2;  // scale * log2 e
+  // the tile kernel's
+  int32_t by_row, page_rows, head_rows, no_row;  // where a page's rows lie in the tensor maps; a row behind the last
+  int32_t part_rows;                             // rows of a block of partial results
+  uint32_t* prefix;                              // [slots + 1] units of work before a slot
+  float2* part_stat;                             // [CTAs][2][part_rows] (maximum in log2, sum)
+  float* part;                                   // [CTAs][2][part_rows][dim]
+};
+
+// How the two groups of softmax warps share the work. kSplit: one tile of rows, the tiles of keys
+// go to the groups in turn, each with sums of its own that meet at the end. kPair: two tiles of rows,
+// one a group, over the same keys. kSingle: one group (at dim 256 the sums of one tile of rows take half
+// of the tensor memory, and two score tiles a part of the rest).
+enum { kSplit = 0, kPair = 1, kSingle = 2 };
+
+template <int DIM, int MODE>
+struct TilePlan {
+  static constexpr int kKeys = DIM == 256 ? 64 : 128;          // keys in a tile: 32 KB at dim 128 and 256
+  static constexpr int kRows = MODE == kPair ? 256 : 128;      // rows of an item
+  static constexpr int kGroups = MODE == kSingle ? 1 : 2;
+  static constexpr int kThreadsT = kGroups * 128 + 128;      // and four warps of which one copies and one issues the products
+  static constexpr int kQBytes = kRows * DIM * 2;
+  static constexpr int kTile = kKeys * DIM * 2;
+  static constexpr int kSlots = DIM == 64 ? 12 : MODE == kSplit ? 6 : 5;  // tiles in the ring: what 227 KB leave beside the queries
+  static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 512;
+  static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
+  static constexpr uint32_t kSums = 256;
+};
+static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kSingle>::kSmem <= 232448 &&
+              TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
+
+struct SlotWork {
+  int off, n, len, end, tiles, blocks, units;  // blocks of rows a key head; units: tiles of keys x blocks x key heads
+  bool bad;
+};
+template <int KEYS, int ROWS>
+__device__ __forceinline__ SlotWork slot_work(const TreeDev& a, int s) {
+  SlotWork w;
+  const int r1 = a.node_off[s + 1], used = a.c.used[s];
+  w.off = a.node_off[s];
+  w.n = r1 - w.off;
+  w.len = a.c.len[s];
+  w.bad = w.off < 0 || r1 < w.off || r1 > a.T || w.n > a.max_nodes ||
+          (w.n > 0 && (w.len < 0 || used < 0 || used > a.c.max_pages || (int64_t)w.len + w.n > ((int64_t)used << a.c.page_shift)));
+  if (w.bad || w.n == 0) {
+    w.n = w.end = w.tiles = w.blocks = w.units = 0;
+    return w;
+  }
+  w.end = w.len + w.n;
+  w.tiles = (w.end + KEYS - 1) / KEYS;
+  w.blocks = (w.n * a.group + ROWS - 1) / ROWS;
+  w.units = w.tiles * w.blocks * a.c.heads;
+  return w;
+}
+
+// All slots' units in a row (slot, key head, block of rows, tile of keys) are dealt out evenly: CTA c of G takes
+// [total c / G, total (c + 1) / G), so the lengths need not be known on the host. An item that lies in
+// one CTA is finished there; one that is cut leaves partial results, joined by join_kernel.
+__device__ __forceinline__ uint32_t first_unit(uint32_t total, int c, int ctas) { return (uint32_t)((uint64_t)total * (uint32_t)c / (uint32_t)ctas); }
+__device__ __forceinline__ int cta_of_unit(uint32_t total, uint32_t u, int ctas) { return (int)(((uint64_t)(u + 1) * (uint32_t)ctas - 1) / total); }
+
+struct Piece {  // of an item: tiles [t0, t1)
+  int head, block, t0, t1;
+};
+template <int KEYS, int ROWS>
+struct Walk {
+  uint32_t u, u1, base;
+  int s;
+  SlotWork w;
+  __device__ __forceinline__ Walk(const TreeDev& a, uint32_t u0_, uint32_t u1_, int s0, uint32_t base0) : u(u0_), u1(u1_), base(base0), s(s0), w(slot_work<KEYS, ROWS>(a, s0)) {}
+  __device__ __forceinline__ bool next(const TreeDev& a, Piece& p) {
+    if (u >= u1) return false;
+    while (u >= base + (uint32_t)w.units) {
+      base += (uint32_t)w.units;
+      ++s;
+      w = slot_work<KEYS, ROWS>(a, s);
+    }
+    const int x = (int)(u - base), item = x / w.tiles;
+    p.head = item / w.blocks;
+    p.block = item - p.head * w.blocks;
+    p.t0 = x - item * w.tiles;
+    p.t1 = min(w.tiles, p.t0 + (int)(u1 - u));
+    u += (uint32_t)(p.t1 - p.t0);
+    return true;
+  }
+};
+
+// Bounded wait; when one runs out, every other wait of the CTA ends too.
+__device__ __forceinline__ uint64_t clock_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool hold(uint64_t* bar, uint32_t parity, volatile int* fail) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t began = clock_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*fail) return false;
+    if (clock_ns() - began > 2000000000ull) break;  // two seconds
+  }
+  *fail = 1;
+  return false;
+}
+__device__ __forceinline__ bool hold_warp(uint64_t* bar, uint32_t parity, volatile int* fail) {
+  return __all_sync(0xFFFFFFFFu, hold(bar, parity, fail));
+}
+
+template <typename T> struct Weight;
+template <> struct Weight<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
+  static constexpr float kShift = 0.0f, kSlack = 8.0f;
+  static constexpr uint32_t kExp = 0x7F80u;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float widen(uint32_t bits) { return __uint_as_float(bits << 16); }
+};
+// fp16 weights are carried 2^11 times as large: a weight of 2^-25 of the largest would else be
+// rounded to nothing, and a hundred thousand of them are not nothing
+template <> struct Weight<__half> {
+  static constexpr bool kBf16 = false;
+  static constexpr float kShift = 11.0f, kSlack = 4.0f;  // 2^15 at most: fp16 ends at 65504
+  static constexpr uint32_t kExp = 0x7C00u;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float widen(uint32_t bits) {
+    const __half h = __ushort_as_half((unsigned short)bits);
+    return __half2float(h);
+  }
+};
+
+// weight * sum, where the weight may have been rounded to nothing and the sum may be infinite
+__device__ __forceinline__ float weighed(float w, float o) { return w == 0.0f ? (fabsf(o) <= 3.402823466e38f ? 0.0f : o) : w * o; }
+
+template <typename T, int DIM, int MODE>
+__global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
+    tree_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeDev a) {
+  using P = TilePlan<DIM, MODE>;
+  using W = Weight<T>;
+  constexpr int kKeys = P::kKeys, kRows = P::kRows, kRing = P::kSlots, kNT = P::kThreadsT;
+  extern __shared__ __align__(1024) char smem[];
+  char* sq = smem;
+  char* ring = smem + P::kQBytes;
+  float2* stat = reinterpret_cast<float2*>(ring + kRing * P::kTile);  // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stat + 256);
+  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_full = s_full + 2, *q_full = p_full + 2, *item_done = q_full + 1, *sums_done = item_done + 1,
+           *stat_full = sums_done + 1, *drain = stat_full + 1;
+  unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this item and the next
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
+  volatile int* fail = reinterpret_cast<volatile int*>(s_tmem + 1);
+  int* s_start = reinterpret_cast<int*>(s_tmem + 2);
+  uint32_t* s_sums = s_tmem + 3;  // [warps]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
+  pdl_trigger();
+  if (smem_addr(smem) & 1023u) {  // (the tiles' swizzle goes by the address)
+    if (cta == 0 && tid == 0) raise_status(a.c.status, ARCS_ERR_CUDA);
+    return;
+  }
+
+  // ---- where this CTA's units begin (the running sum stands where the tiles will come later)
+  uint32_t* pre = reinterpret_cast<uint32_t*>(ring);
+  uint32_t total = 0;
+  for (int s0 = 0; s0 < a.c.slots; s0 += kNT) {
+    const int s = s0 + tid;
+    uint32_t mine = 0;
+    if (s < a.c.slots) {
+      const SlotWork w = slot_work<kKeys, kRows>(a, s);
+      if (w.bad && cta == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
+      mine = (uint32_t)w.units;
+    }
+    uint32_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_sums[warp] = x;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < kNT / 32; ++i) {
+      const uint32_t v = s_sums[i];
+      if (i < warp) before += v;
+      all += v;
+    }
+    if (s < a.c.slots) pre[s] = total + before + x - mine;
+    total += all;
+    __syncthreads();
+  }
+  if (tid == 0) pre[a.c.slots] = total;
+  __syncthreads();
+  if (cta == 0)
+    for (int s = tid; s <= a.c.slots; s += kNT) a.prefix[s] = pre[s];
+  const uint32_t u0 = first_unit(total, cta, ctas), u1 = first_unit(total, cta + 1, ctas);
+  if (u0 == u1) return;
+  for (int s = tid; s < a.c.slots; s += kNT)
+    if (pre[s] <= u0 && u0 < pre[s + 1]) {
+      s_start[0] = s;
+      odd[0] = pre[s];
+    }
+  if (tid == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+    }
+    mbar_init(q_full, P::kGroups * 128);
+    mbar_init(item_done, 1);
+    mbar_init(sums_done, 1);
+    mbar_init(stat_full, P::kGroups * 128);
+    mbar_init(drain, 1);
+    *fail = 0;
+    mbar_init_fence();
+  }
+  if (warp == P::kGroups * 4 + 1) tmem_alloc(s_tmem, 512);
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const int s_first = s_start[0];
+  const uint32_t base_first = (uint32_t)odd[0];
+  const uint32_t tmem = *s_tmem;
+  __syncthreads();
+  if (tid == 0) odd[0] = odd[1] = 0;
+  __syncthreads();
+  Walk<kKeys, kRows> walk(a, u0, u1, s_first, base_first);
+  Piece p;
+
+  // (two groups: 384 threads of 168 registers; the softmax warps take what the other four need not hold)
+  if (warp >= P::kGroups * 4) {
+    if (P::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == P::kGroups * 4) {
+    // ================================================ copies: keys and values of the pieces, in the order in which they are used
+    if (lane == 0) {
+      prefetch_map(&map_k);
+      prefetch_map(&map_v);
+    }
+    const int box = min(a.c.page_size, kKeys);
+    uint32_t rc = 0;
+    bool ok = true;
+    while (ok && walk.next(a, p)) {
+      const int n = p.t1 - p.t0, end = walk.w.end;
+      const int32_t* list = a.c.table + (int64_t)walk.s * a.c.max_pages;
+      // the page that this lane copies of a tile
+      auto page_of = [&](int j) {
+        const int place = (p.t0 + j) * kKeys + lane * box;
+        return j < n && lane * box < kKeys && place < end ? list[place >> a.c.page_shift] : 0;
+      };
+      int id_before = 0, id = 0, id_next = page_of(0);
+      for (int e = 0; e < 2 * n; ++e) {
+        bool is_k;
+        int j;
+        if (MODE == kPair) {
+          is_k = !(e & 1);
+          j = e >> 1;
+        } else {
+          is_k = e == 0 || ((e & 1) && e != 2 * n - 1);
+          j = is_k ? (e + 1) >> 1 : e == 2 * n - 1 ? n - 1 : (e >> 1) - 1;
+        }
+        if (is_k) {
+          id_before = id;
+          id = id_next;
+          id_next = page_of(j + 1);
+        }
+        int pg = is_k || MODE == kPair || e == 2 * n - 1 ? id : id_before;
+        const int slot = rc % kRing;
+        if (!hold_warp(&empty[slot], ((rc / kRing) & 1u) ^ 1u, fail)) {
+          ok = false;
+          break;
+        }
+        const int place = (p.t0 + j) * kKeys, boxes = (min(kKeys, end - place) + box - 1) / box;
+        if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * DIM * 2));
+        __syncwarp();
+        if (lane < boxes) {
+          int row = a.no_row;
+          if (pg >= 0 && pg < a.c.n_pages) row = pg * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
+          else raise_status(a.c.status, ARCS_ERR_PAGE);
+          const int y = a.by_row ? row : p.head, z = a.by_row ? 0 : row;
+          char* dst = ring + slot * P::kTile + lane * box * 128;
+#pragma unroll
+          for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), is_k ? &map_k : &map_v, c * 64, y, z, &full[slot]);
+        }
+        ++rc;
+      }
+    }
+    if (!ok && lane == 0)  // the copies in flight land before the CTA's memory goes to another
+      for (uint32_t i = rc > (uint32_t)kRing ? rc - kRing : 0; i < rc; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
+  } else if (warp == P::kGroups * 4 + 1) {
+    // ================================================ products
+    if (lane == 0) {
+      constexpr uint32_t kScores = mma_desc(128, kKeys, W::kBf16, false), kValues = mma_desc(128, DIM, W::kBf16, true);
+      uint32_t rc = 0, k = 0, turn = 0;  // (turn: a bit a score tile, the phase its barriers are in)
+      bool ok = true;
+      auto scores = [&](int b, int tile, uint32_t at) {  // rows of queries `tile` x the keys in ring slot `at`
+        const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2), ka = smem_addr(ring) + at * P::kTile;
+#pragma unroll
+        for (int i = 0; i < DIM / 16; ++i)
+          mma_ss(tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
+                 i > 0);
+      };
+      auto values = [&](int b, int sums, uint32_t at, bool first) {  // weights of score tile b x the values in ring slot `at`
+        const uint32_t va = smem_addr(ring) + at * P::kTile;
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_ts(tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
+      };
+      while (ok && walk.next(a, p)) {
+        const int n = p.t1 - p.t0;
+        const bool two = MODE == kPair && walk.w.n * a.group - p.block * kRows > 128;
+        ok = hold(q_full, k & 1u, fail);
+        tc_fence_after();
+        uint32_t k_at = 0, v_at = 0;
+        for (int j = 0; ok && j <= n; ++j) {
+          if (MODE == kPair) {
+            if (j >= 1) {
+              v_at = rc % kRing;
+              ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[0], turn & 1u, fail);
+              turn ^= 1u;
+              if (!ok) break;
+              ++rc;
+              tc_fence_after();
+              values(0, 0, v_at, j == 1);
+              if (!two) mma_commit(&empty[v_at]);
+            }
+            if (j < n) {
+              k_at = rc % kRing;
+              ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
+              if (!ok) break;
+              ++rc;
+              scores(0, 0, k_at);
+              mma_commit(&s_full[0]);
+              if (!two) mma_commit(&empty[k_at]);
+            }
+            if (two && j >= 1) {
+              ok = hold(&p_full[1], (turn >> 1) & 1u, fail);
+              turn ^= 2u;
+              if (!ok) break;
+              tc_fence_after();
+              values(1, 1, v_at, j == 1);
+              mma_commit(&empty[v_at]);
+            }
+            if (two && j < n) {
+              scores(1, 1, k_at);
+              mma_commit(&s_full[1]);
+              mma_commit(&empty[k_at]);
+            }
+          } else {
+            if (j < n) {
+              k_at = rc % kRing;
+              ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
+              if (!ok) break;
+              ++rc;
+              scores(j & 1, 0, k_at);
+              mma_commit(&s_full[j & 1]);
+              mma_commit(&empty[k_at]);
+            }
+            if (j >= 1) {
+              const int b = (j - 1) & 1;
+              v_at = rc % kRing;
+              ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[b], (turn >> b) & 1u, fail);
+              turn ^= 1u << b;
+              if (!ok) break;
+              ++rc;
+              tc_fence_after();
+              values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
+              mma_commit(&empty[v_at]);
+              if (MODE == kSingle) mma_commit(sums_done);
+            }
+          }
+        }
+        if (!ok) break;
+        mma_commit(item_done);
+        ++k;
+      }
+      if (!ok) {
+        mma_commit(drain);
+        mbar_wait(drain, 0);
+      }
+    }
+    __syncwarp();
+    }
+  } else {
+    if (P::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ================================================ softmax: a thread a row
+    const int grp = MODE == kSingle ? 0 : warp >> 2, row_t = tid & 127;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes of tensor memory
+    const int first_row = MODE == kPair ? grp * 128 : 0, my = first_row + row_t;
+    const float sl2 = a.scale_log2;
+    uint32_t rc0 = 0, turn = 0, k = 0, done = 0;  // ring position; phases of the score tiles; pieces; tiles (of the one group)
+    bool ok = true;
+    while (ok && walk.next(a, p)) {
+      const int n = p.t1 - p.t0, len = walk.w.len, end = walk.w.end, off = walk.w.off;
+      const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
+      const bool warp_live = first_row + (warp & 3) * 32 < rows, live = my < rows;
+      // ---- queries to shared memory
+      {
+        constexpr int kChunks = DIM / 8, kBy = MODE == kPair ? 128 : P::kGroups * 128;
+        const int have = min(128, rows - first_row);
+        for (int i = MODE == kPair ? row_t : tid; i < have * kChunks; i += kBy) {
+          const int r = i / kChunks, c = i % kChunks, x = p.block * kRows + first_row + r, node = x / a.group, h = p.head * a.group + x - node * a.group;
+          const uint4 v = *reinterpret_cast<const uint4*>(a.q + (off + node) * a.q_token_stride + h * a.q_head_stride + c * 16);
+          *reinterpret_cast<uint4*>(sq + first_row * (DIM * 2) + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        mbar_arrive(q_full);
+      }
+      const int x = p.block * kRows + (live ? my : 0), node = x / a.group, head_q = p.head * a.group + x - node * a.group;
+      unsigned long long bits = 0;
+      if (live) bits = a.mask ? a.mask[off + node] : (2ull << node) - 1ull;
+      if (walk.w.n < 64) bits &= (1ull << walk.w.n) - 1ull;
+
+      float m = -INFINITY, l = 0.0f;  // the reference of this row's weights (at most kSlack below the largest score, in log2), their sum
+      const int mine = MODE == kPair && grp == 1 && rows <= 128 ? 0 : n;
+      for (int j = MODE == kSplit ? grp : 0; j < mine; j += MODE == kSplit ? 2 : 1) {
+        const int b = MODE == kPair ? grp : j & 1;
+        const uint32_t score = lanes + b * P::kScore1;
+        if (!hold_warp(&s_full[b], (turn >> b) & 1u, fail)) {
+          ok = false;
+          break;
+        }
+        turn ^= 1u << b;
+        tc_fence_after();
+        const int p0 = (p.t0 + j) * kKeys;
+        const bool tail = p0 + kKeys > len;
+        if (warp_live) {
+          uint32_t s[kKeys / 32][32];
+#pragma unroll
+          for (int i = 0; i < kKeys / 32; ++i) tmem_ld32(s[i], score + i * 32);
+          tmem_wait_ld();
+          if (tail) {  // column c is place p0 + c: a settled token, a node (its bit decides), or nothing
+#pragma unroll
+            for (int i = 0; i < kKeys / 32; ++i) {
+              const int rel = len - p0 - 32 * i;  // columns of these 32 that are settled tokens
+              const uint32_t settled = rel >= 32 ? ~0u : rel <= 0 ? 0u : (1u << rel) - 1u;
+              const uint32_t nodes = rel >= 32 ? 0u : rel >= 0 ? (uint32_t)(bits << rel) : rel > -64 ? (uint32_t)(bits >> -rel) : 0u;
+              const uint32_t see = settled | nodes;
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!((see >> c) & 1u)) s[i][c] = 0xFF800000u;
+            }
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kKeys / 32; ++i)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(s[i][c]));
+          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+          // The reference moves only when a weight would pass 2^kSlack: the sums rarely have to be
+          // brought down, and nothing is lost, because weights and sums carry the same factor.
+          const bool moves = live && most > m + W::kSlack;
+          if (__any_sync(0xFFFFFFFFu, moves)) {
+            const float f = moves ? exp2_approx(m - most) : 1.0f;
+            if (moves) m = most;
+            l *= f;
+            const bool some = MODE == kSplit ? j >= 2 : j >= 1;  // (there is a sum to bring down)
+            if (some) {
+              if (MODE == kSingle && !hold_warp(sums_done, (done - 1u) & 1u, fail)) {
+                ok = false;
+                break;
+              }
+              if (MODE == kSingle) tc_fence_after();
+              const uint32_t sums = lanes + P::kSums + (MODE == kSingle ? 0 : grp * DIM);
+#pragma unroll
+              for (int i = 0; i < DIM / 32; ++i) {
+                uint32_t o[32];
+                tmem_ld32(o, sums + i * 32);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                tmem_st32(sums + i * 32, o);
+              }
+            }
+          }
+          const float ref = (m == -INFINITY ? 0.0f : m) - W::kShift;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < kKeys / 64; ++i) {
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const float e0 = exp2_approx(fmaf(__uint_as_float(s[2 * i + c / 16][(2 * c) % 32]), sl2, -ref));
+              const float e1 = exp2_approx(fmaf(__uint_as_float(s[2 * i + c / 16][(2 * c + 1) % 32]), sl2, -ref));
+              sum[(2 * c) & 3] += e0;
+              sum[(2 * c + 1) & 3] += e1;
+              w[c] = W::pack(e0, e1);
+            }
+            tmem_st32(score + i * 32, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        if (tail && (MODE != kPair || grp == 0)) {
+          // Values behind the last node are whatever the page holds, and 0 times NaN is NaN: they become
+          // zeros. A node's value that is not finite, too: it is added at the end to the rows that see the node.
+          const uint32_t at = rc0 + (MODE == kPair ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
+          if (!hold_warp(&full[at % kRing], (at / kRing) & 1u, fail)) {
+            ok = false;
+            break;
+          }
+          char* tile = ring + (at % kRing) * P::kTile;
+          const int lo = max(0, len - p0);
+          for (int i = row_t; i < (kKeys - lo) * (DIM / 8); i += 128) {
+            const int r = lo + i / (DIM / 8), c = i % (DIM / 8);
+            uint4* v = reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (c & 7) * 16);
+            if (p0 + r >= end) {
+              *v = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 y = *v;
+            bool hit = false;
+            auto clean = [&](uint32_t w) {
+              if ((w & W::kExp) == W::kExp) { w &= 0xFFFF0000u; hit = true; }
+              if ((w & (W::kExp << 16)) == (W::kExp << 16)) { w &= 0x0000FFFFu; hit = true; }
+              return w;
+            };
+            y = make_uint4(clean(y.x), clean(y.y), clean(y.z), clean(y.w));
+            if (hit) {
+              *v = y;
+              atomicOr(&odd[k & 1u], 1ull << (p0 + r - len));
+            }
+          }
+          fence_proxy_async();
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[b]);
+        ++done;
+      }
+      if (!ok) break;
+
+      // ---- the end of the piece
+      if (!hold_warp(item_done, k & 1u, fail)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (MODE == kSplit) stat[grp * 128 + row_t] = make_float2(m, l);
+      if (P::kGroups == 2) {
+        mbar_arrive(stat_full);
+        if (!hold_warp(stat_full, k & 1u, fail)) {
+          ok = false;
+          break;
+        }
+      }
+      float f0 = 1.0f, f1 = 0.0f;
+      if (MODE == kSplit) {
+        const float2 s0 = stat[row_t], s1 = stat[128 + row_t];
+        m = fmaxf(s0.x, s1.x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        f0 = exp2_approx(s0.x - ref);
+        f1 = exp2_approx(s1.x - ref);
+        l = f0 * s0.y + f1 * s1.y;
+      }
+      if (warp_live && mine > 0) {
+        const bool whole = p.t0 == 0 && p.t1 == walk.w.tiles, sees = l > 0.0f || l != l;
+        const float inv = sees ? 1.0f / l : 0.0f;
+        const int64_t block = ((int64_t)cta * 2 + (p.t0 == 0)) * a.part_rows + my;
+        unsigned long long fix = odd[k & 1u] & bits;
+        constexpr int kCols = MODE == kSplit ? DIM / 2 : DIM;
+        const int c0 = MODE == kSplit ? grp * kCols : 0;
+        if (live && (MODE != kSplit || grp == 0)) {
+          if (!whole) a.part_stat[block] = make_float2(m - W::kShift, l);
+          else if (a.lse) a.lse[(int64_t)(off + node) * a.Hq + head_q] = sees ? (m - W::kShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kCols / 32; ++i) {
+          const int col = c0 + i * 32;
+          uint32_t o[32];
+          tmem_ld32(o, lanes + P::kSums + (MODE == kPair ? grp * DIM : 0) + col);
+          tmem_wait_ld();
+          if (MODE == kSplit) {
+            if (n > 1) {
+              uint32_t o1[32];
+              tmem_ld32(o1, lanes + P::kSums + DIM + col);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(weighed(f0, __uint_as_float(o[c])) + weighed(f1, __uint_as_float(o1[c])));
+            }  // (else the other group has no sums, and f0 is 1 or the row saw nothing)
+          }
+          if (fix) {
+            for (unsigned long long f = fix; f; f &= f - 1) {
+              const int place = len + __ffsll((long long)f) - 1, pg = a.c.table[(int64_t)walk.s * a.c.max_pages + (place >> a.c.page_shift)];
+              if (pg < 0 || pg >= a.c.n_pages) continue;
+              const unsigned short* v = reinterpret_cast<const unsigned short*>(a.c.v + pg * a.c.page_stride + p.head * a.c.head_stride + (place & (a.c.page_size - 1)) * a.c.token_stride) + col;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const uint32_t y = v[c];
+                if ((y & W::kExp) == W::kExp) o[c] = __float_as_uint(__uint_as_float(o[c]) + W::widen(y));
+              }
+            }
+          }
+          if (!live) continue;
+          if (whole) {
+            char* dst = a.out + (off + node) * a.out_token_stride + head_q * a.out_head_stride + col * 2;
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                y[e] = sees ? W::pack(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv) : 0u;
+              *reinterpret_cast<uint4*>(dst + c * 2) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          } else {
+            float* dst = a.part + block * DIM + col;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      if (tid == 0) odd[(k + 1) & 1u] = 0;
+      rc0 += 2 * n;
+      ++k;
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && *fail) raise_status(a.c.status, ARCS_ERR_TIMEOUT);
+  if (warp == P::kGroups * 4 + 1) tmem_free(tmem, 512);
+}
+
+// The pieces of items that were cut, joined: a warp a row, the pieces' weights first (32 at a time), then
+// their sums.
+template <typename T, int DIM, int MODE>
+__global__ void __launch_bounds__(256) join_kernel(const TreeDev a, int ctas) {
+  using P = TilePlan<DIM, MODE>;
+  using W = Weight<T>;
+  constexpr int kPer = DIM / 32;
+  pdl_wait();
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
+  if (t >= a.T) return;
+  const int s = slot_of_row(a.node_off, a.c.slots, t);
+  if (s < 0) return;
+  const SlotWork w = slot_work<P::kKeys, P::kRows>(a, s);
+  if (w.n == 0) return;
+  const int head = h / a.group, r = (t - w.off) * a.group + h % a.group, block = r / P::kRows, rr = r % P::kRows;
+  const uint32_t total = a.prefix[a.c.slots], u = a.prefix[s] + (uint32_t)((head * w.blocks + block) * w.tiles);
+  const int c0 = cta_of_unit(total, u, ctas), c1 = cta_of_unit(total, u + (uint32_t)w.tiles - 1u, ctas);
+  if (c0 == c1) return;
+  float m = -INFINITY, l = 0.0f, o[kPer];
+#pragma unroll
+  for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+  for (int b = c0; b <= c1; b += 32) {
+    const int c = b + lane;
+    const int64_t mine = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
+    float2 st = make_float2(-INFINITY, 0.0f);
+    // (with fewer units than CTAs some of them have none)
+    const bool there = c <= c1 && first_unit(total, c, ctas) != first_unit(total, c + 1, ctas);
+    if (there) st = __ldcg(a.part_stat + mine);
+    float top = st.x;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    const float before = m;
+    m = fmaxf(m, top);
+    const float ref = m == -INFINITY ? 0.0f : m, f = exp2_approx(before - ref), wt = exp2_approx(st.x - ref);
+    float sum = wt * st.y;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    l = weighed(f, l) + sum;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) o[d] = weighed(f, o[d]);
+    const unsigned pieces = __ballot_sync(0xFFFFFFFFu, there);
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      if (!((pieces >> i) & 1u)) continue;
+      const float wi = __shfl_sync(0xFFFFFFFFu, wt, i);
+      const int64_t at = ((int64_t)(b + i) * 2 + (b + i == c0)) * a.part_rows + rr;
+      const float* src = a.part + at * DIM + lane * kPer;
+      float y[kPer];
+      if (kPer == 2) *reinterpret_cast<float2*>(y) = __ldcg(reinterpret_cast<const float2*>(src));
+#pragma unroll
+      for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) o[d] += weighed(wi, y[d]);
+    }
+  }
+  const bool sees = l > 0.0f || l != l;
+  const float inv = sees ? 1.0f / l : 0.0f;
+  char* dst = a.out + t * a.out_token_stride + h * a.out_head_stride + lane * kPer * 2;
+#pragma unroll
+  for (int d = 0; d < kPer; d += 2) *reinterpret_cast<uint32_t*>(dst + d * 2) = sees ? W::pack(o[d] * inv, o[d + 1] * inv) : 0u;
+  if (a.lse && lane == 0) a.lse[(int64_t)t * a.Hq + h] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace arcs
