@@ -109,7 +109,7 @@ bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const Row
 }
 
 constexpr int kCtas = kSmCount;
-int mode_of(int dim, int rows) { return dim == 256 ? kSingle : rows > 128 ? kPair : kSplit; }
+int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair : kSplit; }
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -119,9 +119,11 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a,
   static std::atomic<unsigned long long> attr_done{0};
   const cudaError_t e = ensure_dynamic_smem(tree_tiles_kernel<T, DIM, MODE>, P::kSmem, attr_done);
   if (e != cudaSuccess) return set_error(ARCS_ERR_CUDA, cudaGetErrorString(e));
-  tree_tiles_kernel<T, DIM, MODE><<<kCtas, P::kThreadsT, P::kSmem, st>>>(mk, mv, a);
+  tree_tiles_kernel<T, DIM, MODE><<<kCtas, kTileThreads, P::kSmem, st>>>(mk, mv, a);
   if (int rc = check_launch("tree_attention")) return rc;
-  launch_behind(join_kernel<T, DIM, MODE>, dim3((unsigned)(((int64_t)a.T * a.Hq + 7) / 8)), dim3(256), 0, st, a, kCtas);
+  const int64_t rows = (int64_t)a.T * a.Hq;
+  if (rows <= 1024) launch_behind(join_kernel<T, DIM, MODE, 4>, dim3((unsigned)rows), dim3(kJoinThreads), 0, st, a, kCtas);
+  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(kJoinThreads), 0, st, a, kCtas);
   return check_launch("tree_attention");
 }
 
@@ -194,7 +196,7 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
     a.part = reinterpret_cast<float*>(ws + round16(((size_t)c->slots + 1) * 4) + round16(blocks * 8));
 #define ARCS_LAUNCH(TYPE)                                                                \
   do {                                                                                   \
-    if (c->dim == 256) return launch_tiles<TYPE, 256, kSingle>(mk, mv, a, st);           \
+    if (c->dim == 256) return launch_tiles<TYPE, 256, kShare>(mk, mv, a, st);           \
     if (c->dim == 128 && mode == kPair) return launch_tiles<TYPE, 128, kPair>(mk, mv, a, st); \
     if (c->dim == 128) return launch_tiles<TYPE, 128, kSplit>(mk, mv, a, st);            \
     if (mode == kPair) return launch_tiles<TYPE, 64, kPair>(mk, mv, a, st);              \

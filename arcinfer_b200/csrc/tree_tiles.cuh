@@ -26,25 +26,27 @@ struct TreeDev {
 
 // How the two groups of softmax warps share the work. kSplit: one tile of rows, the tiles of keys
 // go to the groups in turn, each with sums of its own that meet at the end. kPair: two tiles of rows,
-// one a group, over the same keys. kSingle: one group (at dim 256 the sums of one tile of rows take half
-// of the tensor memory, and two score tiles a part of the rest).
-enum { kSplit = 0, kPair = 1, kSingle = 2 };
+// one a group, over the same keys. kShare: as kSplit, with one set of sums (at dim 256 it takes half of
+// the tensor memory): the groups hand the reference of the weights on from tile to tile.
+enum { kSplit = 0, kPair = 1, kShare = 2 };
 
 template <int DIM, int MODE>
 struct TilePlan {
   static constexpr int kKeys = DIM == 256 ? 64 : 128;          // keys in a tile: 32 KB at dim 128 and 256
   static constexpr int kRows = MODE == kPair ? 256 : 128;      // rows of an item
-  static constexpr int kGroups = MODE == kSingle ? 1 : 2;
-  static constexpr int kThreadsT = kGroups * 128 + 128;      // and four warps of which one copies and one issues the products
   static constexpr int kQBytes = kRows * DIM * 2;
   static constexpr int kTile = kKeys * DIM * 2;
-  static constexpr int kSlots = DIM == 64 ? 12 : MODE == kSplit ? 6 : 5;  // tiles in the ring: what 227 KB leave beside the queries
-  static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 512;
+  // tiles in the ring: 160 KB a CTA keep the memory busy (20 MB under way on all of them). kSplit and
+  // kShare leave room beside them for a CTA of join_kernel.
+  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : 5;
+  static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 1024;
   static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
   static constexpr uint32_t kSums = 256;
 };
-static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kSingle>::kSmem <= 232448 &&
+static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kShare>::kSmem <= 232448 &&
               TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
+// 8 softmax warps, one that copies, one that issues the products, two that bring the queries
+constexpr int kTileThreads = 384;
 
 struct SlotWork {
   int off, n, len, end, tiles, blocks, units;  // blocks of rows a key head; units: tiles of keys x blocks x key heads
@@ -156,23 +158,24 @@ template <> struct Weight<__half> {
 __device__ __forceinline__ float weighed(float w, float o) { return w == 0.0f ? (fabsf(o) <= 3.402823466e38f ? 0.0f : o) : w * o; }
 
 template <typename T, int DIM, int MODE>
-__global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
+__global__ void __maxnreg__(152)
     tree_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeDev a) {
   using P = TilePlan<DIM, MODE>;
   using W = Weight<T>;
-  constexpr int kKeys = P::kKeys, kRows = P::kRows, kRing = P::kSlots, kNT = P::kThreadsT;
+  constexpr int kKeys = P::kKeys, kRows = P::kRows, kRing = P::kSlots, kNT = kTileThreads;
   extern __shared__ __align__(1024) char smem[];
   char* sq = smem;
   char* ring = smem + P::kQBytes;
   float2* stat = reinterpret_cast<float2*>(ring + kRing * P::kTile);  // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stat + 256);
-  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_full = s_full + 2, *q_full = p_full + 2, *item_done = q_full + 1, *sums_done = item_done + 1,
-           *stat_full = sums_done + 1, *drain = stat_full + 1;
-  unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this item and the next
+  float* handed = reinterpret_cast<float*>(stat + 256);               // [128] (kShare) the reference after the last tile
+  uint64_t* bars = reinterpret_cast<uint64_t*>(handed + 128);
+  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_full = s_full + 2, *ref_set = p_full + 2 /* [2][4] */, *q_full = ref_set + 8, *q_empty = q_full + 1,
+           *item_done = q_empty + 1, *sums_done = item_done + 1, *stat_full = sums_done + 1, *sums_free = stat_full + 1, *drain = sums_free + 1;
+  unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this piece and the next
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
   volatile int* fail = reinterpret_cast<volatile int*>(s_tmem + 1);
-  int* s_start = reinterpret_cast<int*>(s_tmem + 2);
-  uint32_t* s_sums = s_tmem + 3;  // [warps]
+  uint32_t* s_begin = s_tmem + 2;  // [3] first slot, units before it, units in all
+  uint32_t* s_sums = s_tmem + 5;   // [12]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
   pdl_trigger();
   if (smem_addr(smem) & 1023u) {  // (the tiles' swizzle goes by the address)
@@ -180,255 +183,321 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
     return;
   }
 
-  // ---- where this CTA's units begin (the running sum stands where the tiles will come later)
-  uint32_t* pre = reinterpret_cast<uint32_t*>(ring);
-  uint32_t total = 0;
-  for (int s0 = 0; s0 < a.c.slots; s0 += kNT) {
-    const int s = s0 + tid;
-    uint32_t mine = 0;
-    if (s < a.c.slots) {
-      const SlotWork w = slot_work<kKeys, kRows>(a, s);
-      if (w.bad && cta == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
-      mine = (uint32_t)w.units;
-    }
-    uint32_t x = mine;
+  // ---- where this CTA's units begin. Up to 128 slots every warp adds up on its own, which asks for no
+  // barrier but the one behind the set-up; more are added up by the whole CTA, in the ring's memory.
+  uint32_t total = 0, u0 = 0, u1 = 0, base = 0;
+  int s_first = -1;
+  const bool few = a.c.slots <= 128;
+  uint32_t own[4] = {0, 0, 0, 0};
+  if (few) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_sums[warp] = x;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int i = 0; i < kNT / 32; ++i) {
-      const uint32_t v = s_sums[i];
-      if (i < warp) before += v;
-      all += v;
-    }
-    if (s < a.c.slots) pre[s] = total + before + x - mine;
-    total += all;
-    __syncthreads();
+    for (int i = 0; i < 4; ++i)
+      if (i * 32 < a.c.slots && i * 32 + lane < a.c.slots) {
+        const SlotWork w = slot_work<kKeys, kRows>(a, i * 32 + lane);
+        if (w.bad && cta == 0 && warp == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
+        own[i] = (uint32_t)w.units;
+      }
   }
-  if (tid == 0) pre[a.c.slots] = total;
-  __syncthreads();
-  if (cta == 0)
-    for (int s = tid; s <= a.c.slots; s += kNT) a.prefix[s] = pre[s];
-  const uint32_t u0 = first_unit(total, cta, ctas), u1 = first_unit(total, cta + 1, ctas);
-  if (u0 == u1) return;
-  for (int s = tid; s < a.c.slots; s += kNT)
-    if (pre[s] <= u0 && u0 < pre[s + 1]) {
-      s_start[0] = s;
-      odd[0] = pre[s];
+  if (warp == 9) {
+    tmem_alloc(s_tmem, 512);
+    if (lane == 0) {
+      for (int i = 0; i < kRing; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 128);
+        odd[i] = 0;
+      }
+      for (int i = 0; i < 8; ++i) mbar_init(&ref_set[i], 1);
+      mbar_init(q_full, 64);
+      mbar_init(q_empty, 1);
+      mbar_init(item_done, 1);
+      mbar_init(sums_done, 1);
+      mbar_init(stat_full, 256);
+      mbar_init(sums_free, 256);
+      mbar_init(drain, 1);
+      *fail = 0;
+      mbar_init_fence();
     }
-  if (tid == 0) {
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-    }
-    mbar_init(q_full, P::kGroups * 128);
-    mbar_init(item_done, 1);
-    mbar_init(sums_done, 1);
-    mbar_init(stat_full, P::kGroups * 128);
-    mbar_init(drain, 1);
-    *fail = 0;
-    mbar_init_fence();
   }
-  if (warp == P::kGroups * 4 + 1) tmem_alloc(s_tmem, 512);
-  fence_proxy_async();
+  if (few) {
+    uint32_t before[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i * 32 >= a.c.slots) break;
+      uint32_t x = own[i];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+      }
+      before[i] = total + x - own[i];
+      total += __shfl_sync(0xFFFFFFFFu, x, 31);
+    }
+    u0 = first_unit(total, cta, ctas);
+    u1 = first_unit(total, cta + 1, ctas);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i * 32 >= a.c.slots) break;
+      const unsigned hit = __ballot_sync(0xFFFFFFFFu, before[i] <= u0 && u0 < before[i] + own[i]);
+      if (hit) {
+        s_first = i * 32 + __ffs((int)hit) - 1;
+        base = __shfl_sync(0xFFFFFFFFu, before[i], __ffs((int)hit) - 1);
+      }
+      if (cta == 0 && warp == 0 && i * 32 + lane < a.c.slots) a.prefix[i * 32 + lane] = before[i];
+    }
+    if (cta == 0 && tid == 0) a.prefix[a.c.slots] = total;
+  } else {
+    uint32_t* pre = reinterpret_cast<uint32_t*>(ring);
+    for (int s0 = 0; s0 < a.c.slots; s0 += kNT) {
+      const int s = s0 + tid;
+      uint32_t mine = 0;
+      if (s < a.c.slots) {
+        const SlotWork w = slot_work<kKeys, kRows>(a, s);
+        if (w.bad && cta == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
+        mine = (uint32_t)w.units;
+      }
+      uint32_t x = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_sums[warp] = x;
+      __syncthreads();
+      uint32_t before = 0, all = 0;
+      for (int i = 0; i < kNT / 32; ++i) {
+        const uint32_t v = s_sums[i];
+        if (i < warp) before += v;
+        all += v;
+      }
+      if (s < a.c.slots) pre[s] = total + before + x - mine;
+      total += all;
+      __syncthreads();
+    }
+    if (tid == 0) pre[a.c.slots] = total;
+    __syncthreads();
+    if (cta == 0)
+      for (int s = tid; s <= a.c.slots; s += kNT) a.prefix[s] = pre[s];
+    u0 = first_unit(total, cta, ctas);
+    u1 = first_unit(total, cta + 1, ctas);
+    for (int s = tid; s < a.c.slots; s += kNT)
+      if (pre[s] <= u0 && u0 < pre[s + 1]) {
+        s_begin[0] = (uint32_t)s;
+        s_begin[1] = pre[s];
+      }
+    fence_proxy_async();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int s_first = s_start[0];
-  const uint32_t base_first = (uint32_t)odd[0];
   const uint32_t tmem = *s_tmem;
-  __syncthreads();
-  if (tid == 0) odd[0] = odd[1] = 0;
-  __syncthreads();
-  Walk<kKeys, kRows> walk(a, u0, u1, s_first, base_first);
-  Piece p;
+  if (!few) {
+    s_first = (int)s_begin[0];
+    base = s_begin[1];
+  }
+  if (u0 == u1) {  // nothing for this CTA
+    if (warp == 9) tmem_free(tmem, 512);
+    return;
+  }
 
-  // (two groups: 384 threads of 168 registers; the softmax warps take what the other four need not hold)
-  if (warp >= P::kGroups * 4) {
-    if (P::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == P::kGroups * 4) {
-    // ================================================ copies: keys and values of the pieces, in the order in which they are used
-    if (lane == 0) {
-      prefetch_map(&map_k);
-      prefetch_map(&map_v);
-    }
-    const int box = min(a.c.page_size, kKeys);
-    uint32_t rc = 0;
-    bool ok = true;
-    while (ok && walk.next(a, p)) {
-      const int n = p.t1 - p.t0, end = walk.w.end;
-      const int32_t* list = a.c.table + (int64_t)walk.s * a.c.max_pages;
-      // the page that this lane copies of a tile
-      auto page_of = [&](int j) {
-        const int place = (p.t0 + j) * kKeys + lane * box;
-        return j < n && lane * box < kKeys && place < end ? list[place >> a.c.page_shift] : 0;
-      };
-      int id_before = 0, id = 0, id_next = page_of(0);
-      for (int e = 0; e < 2 * n; ++e) {
-        bool is_k;
-        int j;
-        if (MODE == kPair) {
-          is_k = !(e & 1);
-          j = e >> 1;
-        } else {
-          is_k = e == 0 || ((e & 1) && e != 2 * n - 1);
-          j = is_k ? (e + 1) >> 1 : e == 2 * n - 1 ? n - 1 : (e >> 1) - 1;
-        }
-        if (is_k) {
-          id_before = id;
-          id = id_next;
-          id_next = page_of(j + 1);
-        }
-        int pg = is_k || MODE == kPair || e == 2 * n - 1 ? id : id_before;
-        const int slot = rc % kRing;
-        if (!hold_warp(&empty[slot], ((rc / kRing) & 1u) ^ 1u, fail)) {
-          ok = false;
-          break;
-        }
-        const int place = (p.t0 + j) * kKeys, boxes = (min(kKeys, end - place) + box - 1) / box;
-        if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * DIM * 2));
-        __syncwarp();
-        if (lane < boxes) {
-          int row = a.no_row;
-          if (pg >= 0 && pg < a.c.n_pages) row = pg * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
-          else raise_status(a.c.status, ARCS_ERR_PAGE);
-          const int y = a.by_row ? row : p.head, z = a.by_row ? 0 : row;
-          char* dst = ring + slot * P::kTile + lane * box * 128;
-#pragma unroll
-          for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), is_k ? &map_k : &map_v, c * 64, y, z, &full[slot]);
-        }
-        ++rc;
-      }
-    }
-    if (!ok && lane == 0)  // the copies in flight land before the CTA's memory goes to another
-      for (uint32_t i = rc > (uint32_t)kRing ? rc - kRing : 0; i < rc; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
-  } else if (warp == P::kGroups * 4 + 1) {
-    // ================================================ products
-    if (lane == 0) {
-      constexpr uint32_t kScores = mma_desc(128, kKeys, W::kBf16, false), kValues = mma_desc(128, DIM, W::kBf16, true);
-      uint32_t rc = 0, k = 0, turn = 0;  // (turn: a bit a score tile, the phase its barriers are in)
+  // (384 threads of 152 registers at the start; the softmax warps take what the other four need not hold)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+      // ============================================== copies: keys and values of the pieces, in the order in which they are used
+      const int box = min(a.c.page_size, kKeys);
+      Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
+      Piece p;
+      uint32_t rc = 0;
       bool ok = true;
-      auto scores = [&](int b, int tile, uint32_t at) {  // rows of queries `tile` x the keys in ring slot `at`
-        const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2), ka = smem_addr(ring) + at * P::kTile;
-#pragma unroll
-        for (int i = 0; i < DIM / 16; ++i)
-          mma_ss(tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
-                 i > 0);
-      };
-      auto values = [&](int b, int sums, uint32_t at, bool first) {  // weights of score tile b x the values in ring slot `at`
-        const uint32_t va = smem_addr(ring) + at * P::kTile;
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_ts(tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
-      };
       while (ok && walk.next(a, p)) {
-        const int n = p.t1 - p.t0;
-        const bool two = MODE == kPair && walk.w.n * a.group - p.block * kRows > 128;
-        ok = hold(q_full, k & 1u, fail);
-        tc_fence_after();
-        uint32_t k_at = 0, v_at = 0;
-        for (int j = 0; ok && j <= n; ++j) {
+        const int n = p.t1 - p.t0, end = walk.w.end;
+        const int32_t* list = a.c.table + (int64_t)walk.s * a.c.max_pages;
+        // the page that this lane copies of a tile
+        auto page_of = [&](int j) {
+          const int place = (p.t0 + j) * kKeys + lane * box;
+          return j < n && lane * box < kKeys && place < end ? list[place >> a.c.page_shift] : 0;
+        };
+        int id_before = 0, id = 0, id_next = page_of(0);
+        for (int e = 0; e < 2 * n; ++e) {
+          bool is_k;
+          int j;
           if (MODE == kPair) {
-            if (j >= 1) {
-              v_at = rc % kRing;
-              ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[0], turn & 1u, fail);
-              turn ^= 1u;
-              if (!ok) break;
-              ++rc;
-              tc_fence_after();
-              values(0, 0, v_at, j == 1);
-              if (!two) mma_commit(&empty[v_at]);
-            }
-            if (j < n) {
-              k_at = rc % kRing;
-              ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
-              if (!ok) break;
-              ++rc;
-              scores(0, 0, k_at);
-              mma_commit(&s_full[0]);
-              if (!two) mma_commit(&empty[k_at]);
-            }
-            if (two && j >= 1) {
-              ok = hold(&p_full[1], (turn >> 1) & 1u, fail);
-              turn ^= 2u;
-              if (!ok) break;
-              tc_fence_after();
-              values(1, 1, v_at, j == 1);
-              mma_commit(&empty[v_at]);
-            }
-            if (two && j < n) {
-              scores(1, 1, k_at);
-              mma_commit(&s_full[1]);
-              mma_commit(&empty[k_at]);
-            }
+            is_k = !(e & 1);
+            j = e >> 1;
           } else {
-            if (j < n) {
-              k_at = rc % kRing;
-              ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
-              if (!ok) break;
-              ++rc;
-              scores(j & 1, 0, k_at);
-              mma_commit(&s_full[j & 1]);
-              mma_commit(&empty[k_at]);
-            }
-            if (j >= 1) {
-              const int b = (j - 1) & 1;
-              v_at = rc % kRing;
-              ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[b], (turn >> b) & 1u, fail);
-              turn ^= 1u << b;
-              if (!ok) break;
-              ++rc;
-              tc_fence_after();
-              values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
-              mma_commit(&empty[v_at]);
-              if (MODE == kSingle) mma_commit(sums_done);
+            is_k = e == 0 || ((e & 1) && e != 2 * n - 1);
+            j = is_k ? (e + 1) >> 1 : e == 2 * n - 1 ? n - 1 : (e >> 1) - 1;
+          }
+          if (is_k) {
+            id_before = id;
+            id = id_next;
+            id_next = page_of(j + 1);
+          }
+          const int pg = is_k || MODE == kPair || e == 2 * n - 1 ? id : id_before;
+          const int slot = rc % kRing;
+          if (!hold_warp(&empty[slot], ((rc / kRing) & 1u) ^ 1u, fail)) {
+            ok = false;
+            break;
+          }
+          const int place = (p.t0 + j) * kKeys, boxes = (min(kKeys, end - place) + box - 1) / box;
+          if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * DIM * 2));
+          __syncwarp();
+          if (lane < boxes) {
+            int row = a.no_row;
+            if (pg >= 0 && pg < a.c.n_pages) row = pg * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
+            else raise_status(a.c.status, ARCS_ERR_PAGE);
+            const int y = a.by_row ? row : p.head, z = a.by_row ? 0 : row;
+            char* dst = ring + slot * P::kTile + lane * box * 128;
+#pragma unroll
+            for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), is_k ? &map_k : &map_v, c * 64, y, z, &full[slot]);
+          }
+          ++rc;
+        }
+      }
+      if (!ok && lane == 0)  // the copies in flight land before the CTA's memory goes to another
+        for (uint32_t i = rc > (uint32_t)kRing ? rc - kRing : 0; i < rc; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
+    } else if (warp == 9) {
+      // ============================================== products
+      if (lane == 0) {
+        constexpr uint32_t kScores = mma_desc(128, kKeys, W::kBf16, false), kValues = mma_desc(128, DIM, W::kBf16, true);
+        Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
+        Piece p;
+        uint32_t rc = 0, k = 0, turn = 0;  // (turn: a bit a score tile, the phase its barriers are in)
+        bool ok = true;
+        auto scores = [&](int b, int tile, uint32_t at) {  // rows of queries `tile` x the keys in ring slot `at`
+          const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2), ka = smem_addr(ring) + at * P::kTile;
+#pragma unroll
+          for (int i = 0; i < DIM / 16; ++i)
+            mma_ss(tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
+                   i > 0);
+        };
+        auto values = [&](int b, int sums, uint32_t at, bool first) {  // weights of score tile b x the values in ring slot `at`
+          const uint32_t va = smem_addr(ring) + at * P::kTile;
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
+        };
+        while (ok && walk.next(a, p)) {
+          const int n = p.t1 - p.t0;
+          const bool two = MODE == kPair && walk.w.n * a.group - p.block * kRows > 128;
+          ok = hold(q_full, k & 1u, fail);
+          tc_fence_after();
+          uint32_t k_at = 0, v_at = 0;
+          for (int j = 0; ok && j <= n; ++j) {
+            // (the sums of the piece before have been read: asked before the first product into them)
+            if (j == 1 && k > 0 && !(ok = hold(sums_free, (k - 1u) & 1u, fail))) break;
+            if (MODE == kPair) {
+              if (j >= 1) {
+                v_at = rc % kRing;
+                ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[0], turn & 1u, fail);
+                if (!ok) break;
+                turn ^= 1u;
+                ++rc;
+                tc_fence_after();
+                values(0, 0, v_at, j == 1);
+                if (!two) mma_commit(&empty[v_at]);
+              }
+              if (j < n) {
+                k_at = rc % kRing;
+                ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
+                if (!ok) break;
+                ++rc;
+                scores(0, 0, k_at);
+                mma_commit(&s_full[0]);
+                if (!two) mma_commit(&empty[k_at]);
+                if (!two && j == n - 1) mma_commit(q_empty);
+              }
+              if (two && j >= 1) {
+                ok = hold(&p_full[1], (turn >> 1) & 1u, fail);
+                if (!ok) break;
+                turn ^= 2u;
+                tc_fence_after();
+                values(1, 1, v_at, j == 1);
+                mma_commit(&empty[v_at]);
+              }
+              if (two && j < n) {
+                scores(1, 1, k_at);
+                mma_commit(&s_full[1]);
+                mma_commit(&empty[k_at]);
+                if (j == n - 1) mma_commit(q_empty);
+              }
+            } else {
+              if (j < n) {
+                k_at = rc % kRing;
+                ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
+                if (!ok) break;
+                ++rc;
+                scores(j & 1, 0, k_at);
+                mma_commit(&s_full[j & 1]);
+                mma_commit(&empty[k_at]);
+                if (j == n - 1) mma_commit(q_empty);
+              }
+              if (j >= 1) {
+                const int b = (j - 1) & 1;
+                v_at = rc % kRing;
+                ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[b], (turn >> b) & 1u, fail);
+                if (!ok) break;
+                turn ^= 1u << b;
+                ++rc;
+                tc_fence_after();
+                values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
+                mma_commit(&empty[v_at]);
+                if (MODE == kShare) mma_commit(sums_done);
+              }
             }
           }
+          if (!ok) break;
+          mma_commit(item_done);
+          ++k;
         }
-        if (!ok) break;
-        mma_commit(item_done);
+        if (!ok) {
+          mma_commit(drain);
+          mbar_wait(drain, 0);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ============================================== queries of the next piece, once the products have done with those of this one
+      Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
+      Piece p;
+      const int at = tid - 320;
+      uint32_t k = 0;
+      while (walk.next(a, p)) {
+        if (k > 0 && !hold_warp(q_empty, (k - 1u) & 1u, fail)) break;
+        constexpr int kChunks = DIM / 8;
+        const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
+        const char* from = a.q + walk.w.off * a.q_token_stride;
+        for (int i = at; i < rows * kChunks; i += 64) {
+          const int r = i / kChunks, c = i % kChunks, x = p.block * kRows + r, node = x / a.group, h = p.head * a.group + x - node * a.group;
+          copy16(sq + (r >> 7) * (128 * DIM * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), from + node * a.q_token_stride + h * a.q_head_stride + c * 16);
+        }
+        copy16_wait();
+        fence_proxy_async();
+        mbar_arrive(q_full);
         ++k;
       }
-      if (!ok) {
-        mma_commit(drain);
-        mbar_wait(drain, 0);
-      }
-    }
-    __syncwarp();
     }
   } else {
-    if (P::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ================================================ softmax: a thread a row
-    const int grp = MODE == kSingle ? 0 : warp >> 2, row_t = tid & 127;
+    Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
+    Piece p;
+    const int grp = warp >> 2, row_t = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes of tensor memory
     const int first_row = MODE == kPair ? grp * 128 : 0, my = first_row + row_t;
     const float sl2 = a.scale_log2;
-    uint32_t rc0 = 0, turn = 0, k = 0, done = 0;  // ring position; phases of the score tiles; pieces; tiles (of the one group)
+    const uint64_t scale2 = pair_of(sl2, sl2);
+    // ring position; phase of the score tile; pieces; (kShare) tiles of both groups, references that the other group has set
+    uint32_t rc0 = 0, turn = 0, k = 0, done = 0, set = 0;
     bool ok = true;
     while (ok && walk.next(a, p)) {
       const int n = p.t1 - p.t0, len = walk.w.len, end = walk.w.end, off = walk.w.off;
       const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
       const bool warp_live = first_row + (warp & 3) * 32 < rows, live = my < rows;
-      // ---- queries to shared memory
-      {
-        constexpr int kChunks = DIM / 8, kBy = MODE == kPair ? 128 : P::kGroups * 128;
-        const int have = min(128, rows - first_row);
-        for (int i = MODE == kPair ? row_t : tid; i < have * kChunks; i += kBy) {
-          const int r = i / kChunks, c = i % kChunks, x = p.block * kRows + first_row + r, node = x / a.group, h = p.head * a.group + x - node * a.group;
-          const uint4 v = *reinterpret_cast<const uint4*>(a.q + (off + node) * a.q_token_stride + h * a.q_head_stride + c * 16);
-          *reinterpret_cast<uint4*>(sq + first_row * (DIM * 2) + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-        }
-        fence_proxy_async();
-        mbar_arrive(q_full);
-      }
       const int x = p.block * kRows + (live ? my : 0), node = x / a.group, head_q = p.head * a.group + x - node * a.group;
       unsigned long long bits = 0;
       if (live) bits = a.mask ? a.mask[off + node] : (2ull << node) - 1ull;
@@ -436,14 +505,13 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
 
       float m = -INFINITY, l = 0.0f;  // the reference of this row's weights (at most kSlack below the largest score, in log2), their sum
       const int mine = MODE == kPair && grp == 1 && rows <= 128 ? 0 : n;
-      for (int j = MODE == kSplit ? grp : 0; j < mine; j += MODE == kSplit ? 2 : 1) {
-        const int b = MODE == kPair ? grp : j & 1;
-        const uint32_t score = lanes + b * P::kScore1;
-        if (!hold_warp(&s_full[b], (turn >> b) & 1u, fail)) {
+      for (int j = MODE == kPair ? 0 : grp; j < mine; j += MODE == kPair ? 1 : 2) {
+        const uint32_t score = lanes + grp * P::kScore1;
+        if (!hold_warp(&s_full[grp], turn & 1u, fail)) {
           ok = false;
           break;
         }
-        turn ^= 1u << b;
+        turn ^= 1u;
         tc_fence_after();
         const int p0 = (p.t0 + j) * kKeys;
         const bool tail = p0 + kKeys > len;
@@ -452,6 +520,8 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
 #pragma unroll
           for (int i = 0; i < kKeys / 32; ++i) tmem_ld32(s[i], score + i * 32);
           tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < kKeys / 32; ++i) tmem_use(s[i]);
           if (tail) {  // column c is place p0 + c: a settled token, a node (its bit decides), or nothing
 #pragma unroll
             for (int i = 0; i < kKeys / 32; ++i) {
@@ -468,50 +538,79 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
 #pragma unroll
           for (int i = 0; i < kKeys / 32; ++i)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(s[i][c]));
-          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+            for (int c = 0; c < 32; c += 2) top[(c >> 1) & 3] = max3(top[(c >> 1) & 3], __uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
+          const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * sl2;
           // The reference moves only when a weight would pass 2^kSlack: the sums rarely have to be
           // brought down, and nothing is lost, because weights and sums carry the same factor.
-          const bool moves = live && most > m + W::kSlack;
+          float before = m;
+          if (MODE == kShare && j > 0) {
+            if (!hold_warp(&ref_set[(grp ^ 1) * 4 + (warp & 3)], set++ & 1u, fail)) {
+              ok = false;
+              break;
+            }
+            before = handed[row_t];
+          }
+          const bool moves = live && most > before + W::kSlack;
+          const float now = moves ? most : before;
+          if (MODE == kShare) {
+            handed[row_t] = now;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ref_set[grp * 4 + (warp & 3)]);
+          }
+          if (__any_sync(0xFFFFFFFFu, now != m)) {
+            l *= now != m ? exp2_approx(m - now) : 1.0f;
+            m = now;
+          }
           if (__any_sync(0xFFFFFFFFu, moves)) {
-            const float f = moves ? exp2_approx(m - most) : 1.0f;
-            if (moves) m = most;
-            l *= f;
             const bool some = MODE == kSplit ? j >= 2 : j >= 1;  // (there is a sum to bring down)
             if (some) {
-              if (MODE == kSingle && !hold_warp(sums_done, (done - 1u) & 1u, fail)) {
-                ok = false;
-                break;
+              if (MODE == kShare) {
+                if (!hold_warp(sums_done, (done + j - 1u) & 1u, fail)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
               }
-              if (MODE == kSingle) tc_fence_after();
-              const uint32_t sums = lanes + P::kSums + (MODE == kSingle ? 0 : grp * DIM);
-#pragma unroll
+              const float f = moves ? exp2_approx(before - now) : 1.0f;
+              const uint64_t f2 = pair_of(f, f);
+              const uint32_t sums = lanes + P::kSums + (MODE == kShare ? 0 : grp * DIM);
+#pragma unroll 1
               for (int i = 0; i < DIM / 32; ++i) {
                 uint32_t o[32];
                 tmem_ld32(o, sums + i * 32);
                 tmem_wait_ld();
+                tmem_use(o);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                for (int c = 0; c < 32; c += 2) {
+                  float y0, y1;
+                  pair_out(mul_pair(pair_of(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), f2), y0, y1);
+                  o[c] = __float_as_uint(y0);
+                  o[c + 1] = __float_as_uint(y1);
+                }
                 tmem_st32(sums + i * 32, o);
               }
             }
           }
-          const float ref = (m == -INFINITY ? 0.0f : m) - W::kShift;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float ref = W::kShift - (m == -INFINITY ? 0.0f : m);
+          const uint64_t ref2 = pair_of(ref, ref);
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-          for (int i = 0; i < kKeys / 64; ++i) {
-            uint32_t w[32];
+          for (int i = 0; i < kKeys / 32; ++i) {
+            uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float e0 = exp2_approx(fmaf(__uint_as_float(s[2 * i + c / 16][(2 * c) % 32]), sl2, -ref));
-              const float e1 = exp2_approx(fmaf(__uint_as_float(s[2 * i + c / 16][(2 * c + 1) % 32]), sl2, -ref));
-              sum[(2 * c) & 3] += e0;
-              sum[(2 * c + 1) & 3] += e1;
-              w[c] = W::pack(e0, e1);
+            for (int c = 0; c < 32; c += 2) {
+              float e0, e1;
+              pair_out(fma_pair(pair_of(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])), scale2, ref2), e0, e1);
+              e0 = exp2_approx(e0);
+              e1 = exp2_approx(e1);
+              sum[(c >> 1) & 1] = add_pair(sum[(c >> 1) & 1], pair_of(e0, e1));
+              w[c >> 1] = W::pack(e0, e1);
             }
-            tmem_st32(score + i * 32, w);
+            tmem_st16(score + i * 16, w);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float l0, l1;
+          pair_out(add_pair(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
           tmem_wait_st();
         }
         if (tail && (MODE != kPair || grp == 0)) {
@@ -547,8 +646,7 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
           fence_proxy_async();
         }
         tc_fence_before();
-        mbar_arrive(&p_full[b]);
-        ++done;
+        mbar_arrive(&p_full[grp]);
       }
       if (!ok) break;
 
@@ -558,16 +656,14 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
         break;
       }
       tc_fence_after();
-      if (MODE == kSplit) stat[grp * 128 + row_t] = make_float2(m, l);
-      if (P::kGroups == 2) {
-        mbar_arrive(stat_full);
-        if (!hold_warp(stat_full, k & 1u, fail)) {
-          ok = false;
-          break;
-        }
+      if (MODE != kPair) stat[grp * 128 + row_t] = make_float2(m, l);
+      mbar_arrive(stat_full);
+      if (!hold_warp(stat_full, k & 1u, fail)) {
+        ok = false;
+        break;
       }
       float f0 = 1.0f, f1 = 0.0f;
-      if (MODE == kSplit) {
+      if (MODE != kPair) {
         const float2 s0 = stat[row_t], s1 = stat[128 + row_t];
         m = fmaxf(s0.x, s1.x);
         const float ref = m == -INFINITY ? 0.0f : m;
@@ -579,33 +675,35 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
         const bool whole = p.t0 == 0 && p.t1 == walk.w.tiles, sees = l > 0.0f || l != l;
         const float inv = sees ? 1.0f / l : 0.0f;
         const int64_t block = ((int64_t)cta * 2 + (p.t0 == 0)) * a.part_rows + my;
-        unsigned long long fix = odd[k & 1u] & bits;
-        constexpr int kCols = MODE == kSplit ? DIM / 2 : DIM;
-        const int c0 = MODE == kSplit ? grp * kCols : 0;
-        if (live && (MODE != kSplit || grp == 0)) {
+        const unsigned long long fix = odd[k & 1u] & bits;
+        constexpr int kCols = MODE == kPair ? DIM : DIM / 2;
+        const int c0 = MODE == kPair ? 0 : grp * kCols;
+        if (live && (MODE == kPair || grp == 0)) {
           if (!whole) a.part_stat[block] = make_float2(m - W::kShift, l);
           else if (a.lse) a.lse[(int64_t)(off + node) * a.Hq + head_q] = sees ? (m - W::kShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kCols / 32; ++i) {
           const int col = c0 + i * 32;
           uint32_t o[32];
           tmem_ld32(o, lanes + P::kSums + (MODE == kPair ? grp * DIM : 0) + col);
-          tmem_wait_ld();
-          if (MODE == kSplit) {
-            if (n > 1) {
-              uint32_t o1[32];
-              tmem_ld32(o1, lanes + P::kSums + DIM + col);
-              tmem_wait_ld();
+          if (MODE == kSplit && n > 1) {  // (with one tile the other group has no sums, and f0 is 1 or the row saw nothing)
+            uint32_t o1[32];
+            tmem_ld32(o1, lanes + P::kSums + DIM + col);
+            tmem_wait_ld();
+            tmem_use(o);
+            tmem_use(o1);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(weighed(f0, __uint_as_float(o[c])) + weighed(f1, __uint_as_float(o1[c])));
-            }  // (else the other group has no sums, and f0 is 1 or the row saw nothing)
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(weighed(f0, __uint_as_float(o[c])) + weighed(f1, __uint_as_float(o1[c])));
           }
+          tmem_wait_ld();
+          tmem_use(o);
           if (fix) {
             for (unsigned long long f = fix; f; f &= f - 1) {
               const int place = len + __ffsll((long long)f) - 1, pg = a.c.table[(int64_t)walk.s * a.c.max_pages + (place >> a.c.page_shift)];
               if (pg < 0 || pg >= a.c.n_pages) continue;
-              const unsigned short* v = reinterpret_cast<const unsigned short*>(a.c.v + pg * a.c.page_stride + p.head * a.c.head_stride + (place & (a.c.page_size - 1)) * a.c.token_stride) + col;
+              const unsigned short* v =
+                  reinterpret_cast<const unsigned short*>(a.c.v + pg * a.c.page_stride + p.head * a.c.head_stride + (place & (a.c.page_size - 1)) * a.c.token_stride) + col;
 #pragma unroll
               for (int c = 0; c < 32; ++c) {
                 const uint32_t y = v[c];
@@ -613,8 +711,7 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
               }
             }
           }
-          if (!live) continue;
-          if (whole) {
+          if (live && whole) {
             char* dst = a.out + (off + node) * a.out_token_stride + head_q * a.out_head_stride + col * 2;
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
@@ -624,79 +721,124 @@ __global__ void __launch_bounds__(TilePlan<DIM, MODE>::kThreadsT, 1)
                 y[e] = sees ? W::pack(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv) : 0u;
               *reinterpret_cast<uint4*>(dst + c * 2) = make_uint4(y[0], y[1], y[2], y[3]);
             }
-          } else {
+          } else if (live) {
             float* dst = a.part + block * DIM + col;
 #pragma unroll
             for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
           }
+          __syncwarp();
         }
       }
-      tc_fence_before();
       if (tid == 0) odd[(k + 1) & 1u] = 0;
+      tc_fence_before();
+      mbar_arrive(sums_free);
       rc0 += 2 * n;
+      done += n;
+      if (MODE == kShare && warp_live && (n & 1) == grp && n > grp) ++set;  // (the piece's last tile was the other group's: nobody asked for its reference)
       ++k;
     }
   }
   __syncthreads();
   if (tid == 0 && *fail) raise_status(a.c.status, ARCS_ERR_TIMEOUT);
-  if (warp == P::kGroups * 4 + 1) tmem_free(tmem, 512);
+  if (warp == 9) tmem_free(tmem, 512);
 }
 
-// The pieces of items that were cut, joined: a warp a row, the pieces' weights first (32 at a time), then
-// their sums.
-template <typename T, int DIM, int MODE>
-__global__ void __launch_bounds__(256) join_kernel(const TreeDev a, int ctas) {
+// The pieces of items that were cut, joined. A CTA of four warps takes a row (WARPS = 4: there are few, and
+// each may have a hundred pieces) or four; a warp asks for four pieces' sums at a time, weights beside
+// them. Small enough (56 registers, 128 threads) to be on the SM, its way found, while the last pieces are
+// still worked on.
+constexpr int kJoinThreads = 128;
+template <typename T, int DIM, int MODE, int WARPS>
+__global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, int ctas) {
   using P = TilePlan<DIM, MODE>;
   using W = Weight<T>;
   constexpr int kPer = DIM / 32;
-  pdl_wait();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  __shared__ float2 s_stat[4];
+  __shared__ float s_sum[WARPS == 4 ? 4 : 1][WARPS == 4 ? DIM : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = WARPS == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + warp;
   const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
-  if (t >= a.T) return;
-  const int s = slot_of_row(a.node_off, a.c.slots, t);
-  if (s < 0) return;
-  const SlotWork w = slot_work<P::kKeys, P::kRows>(a, s);
+  const int s = t < a.T ? slot_of_row(a.node_off, a.c.slots, t) : -1;
+  SlotWork w;
+  w.n = 0;
+  if (s >= 0) w = slot_work<P::kKeys, P::kRows>(a, s);
   if (w.n == 0) return;
   const int head = h / a.group, r = (t - w.off) * a.group + h % a.group, block = r / P::kRows, rr = r % P::kRows;
-  const uint32_t total = a.prefix[a.c.slots], u = a.prefix[s] + (uint32_t)((head * w.blocks + block) * w.tiles);
+  uint32_t total = 0, before = 0;
+  if (a.c.slots <= 128) {
+    for (int i = lane; i < a.c.slots; i += 32) {
+      const uint32_t u = (uint32_t)slot_work<P::kKeys, P::kRows>(a, i).units;
+      total += u;
+      if (i < s) before += u;
+    }
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    pdl_wait();
+  } else {
+    pdl_wait();
+    total = __ldcg(a.prefix + a.c.slots);
+    before = __ldcg(a.prefix + s);
+  }
+  const uint32_t u = before + (uint32_t)((head * w.blocks + block) * w.tiles);
   const int c0 = cta_of_unit(total, u, ctas), c1 = cta_of_unit(total, u + (uint32_t)w.tiles - 1u, ctas);
   if (c0 == c1) return;
   float m = -INFINITY, l = 0.0f, o[kPer];
 #pragma unroll
   for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
-  for (int b = c0; b <= c1; b += 32) {
-    const int c = b + lane;
-    const int64_t mine = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
-    float2 st = make_float2(-INFINITY, 0.0f);
-    // (with fewer units than CTAs some of them have none)
-    const bool there = c <= c1 && first_unit(total, c, ctas) != first_unit(total, c + 1, ctas);
-    if (there) st = __ldcg(a.part_stat + mine);
-    float top = st.x;
+  constexpr int kAtOnce = DIM == 256 ? 2 : 4;
+  for (int b = c0 + (WARPS == 4 ? warp : 0) * kAtOnce; b <= c1; b += kAtOnce * WARPS) {
+    float y[kAtOnce][kPer];
+    float2 st[kAtOnce];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    const float before = m;
-    m = fmaxf(m, top);
-    const float ref = m == -INFINITY ? 0.0f : m, f = exp2_approx(before - ref), wt = exp2_approx(st.x - ref);
-    float sum = wt * st.y;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = b + i;
+      // (with fewer units than CTAs some of them have none)
+      const bool there = c <= c1 && first_unit(total, c, ctas) != first_unit(total, c + 1, ctas);
+      const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
+      st[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    l = weighed(f, l) + sum;
+      for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
+      if (there) {
+        const float* src = a.part + at * DIM + lane * kPer;
+        st[i] = __ldcg(a.part_stat + at);
+        if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+#pragma unroll
+        for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
+    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    m = top;
+    l = weighed(f, l);
 #pragma unroll
     for (int d = 0; d < kPer; ++d) o[d] = weighed(f, o[d]);
-    const unsigned pieces = __ballot_sync(0xFFFFFFFFu, there);
-#pragma unroll 4
-    for (int i = 0; i < 32; ++i) {
-      if (!((pieces >> i) & 1u)) continue;
-      const float wi = __shfl_sync(0xFFFFFFFFu, wt, i);
-      const int64_t at = ((int64_t)(b + i) * 2 + (b + i == c0)) * a.part_rows + rr;
-      const float* src = a.part + at * DIM + lane * kPer;
-      float y[kPer];
-      if (kPer == 2) *reinterpret_cast<float2*>(y) = __ldcg(reinterpret_cast<const float2*>(src));
 #pragma unroll
-      for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float wt = exp2_approx(st[i].x - ref);
+      l += wt * st[i].y;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) o[d] += weighed(wi, y[d]);
+      for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, y[i][d]);
+    }
+  }
+  if (WARPS == 4) {  // the four warps' shares: a quarter of the row each
+    if (lane == 0) s_stat[warp] = make_float2(m, l);
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) s_sum[warp][lane * kPer + d] = o[d];
+    __syncthreads();
+    m = fmaxf(fmaxf(s_stat[0].x, s_stat[1].x), fmaxf(s_stat[2].x, s_stat[3].x));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+    if (warp != 0) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float wt = exp2_approx(s_stat[i].x - ref);
+      l += weighed(wt, s_stat[i].y);
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, s_sum[i][lane * kPer + d]);
     }
   }
   const bool sees = l > 0.0f || l != l;
