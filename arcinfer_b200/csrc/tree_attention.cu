@@ -110,6 +110,7 @@ bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const Row
 
 constexpr int kCtas = kSmCount;
 int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair : kSplit; }
+int keys_of(int dim, int mode) { return dim == 256 ? 64 : 128; }
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -178,7 +179,7 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
 
   RowPlan r;
   if (plan_rows(c, &r)) {
-    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = c->dim == 256 ? 64 : 128;
+    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = keys_of(c->dim, mode);
     if ((((int64_t)c->max_pages * c->page_size + keys - 1) / keys) * c->slots * c->heads * ((rows + most - 1) / most) > 0x7FFFFFFFll)
       return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
     if (!encode_tiled()) return set_error(ARCS_ERR_CUDA, "tree_attention: the driver makes no tensor maps");

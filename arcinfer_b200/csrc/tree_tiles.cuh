@@ -32,20 +32,20 @@ enum { kSplit = 0, kPair = 1, kShare = 2 };
 
 template <int DIM, int MODE>
 struct TilePlan {
-  static constexpr int kKeys = DIM == 256 ? 64 : 128;          // keys in a tile: 32 KB at dim 128 and 256
+  static constexpr int kKeys = DIM == 256 ? 64 : 128;
   static constexpr int kRows = MODE == kPair ? 256 : 128;      // rows of an item
   static constexpr int kQBytes = kRows * DIM * 2;
   static constexpr int kTile = kKeys * DIM * 2;
   // tiles in the ring: 160 KB a CTA keep the memory busy (20 MB under way on all of them). kSplit and
   // kShare leave room beside them for a CTA of join_kernel.
-  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : 5;
+  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : MODE == kSplit ? 5 : 5;
   static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 1024;
   static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
   static constexpr uint32_t kSums = 256;
 };
 static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kShare>::kSmem <= 232448 &&
               TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
-// 8 softmax warps, one that copies, one that issues the products, two that bring the queries
+// 8 softmax warps, two that copy keys and values, one that issues the products, one that brings the queries
 constexpr int kTileThreads = 384;
 
 struct SlotWork {
@@ -127,6 +127,12 @@ __device__ __forceinline__ bool hold_warp(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xFFFFFFFFu, hold(bar, parity, fail));
 }
 
+// one arrival for a whole warp's work (the arrivals of a barrier are taken one after the other)
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 template <typename T> struct Weight;
 template <> struct Weight<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
@@ -169,7 +175,7 @@ __global__ void __maxnreg__(152)
   float2* stat = reinterpret_cast<float2*>(ring + kRing * P::kTile);  // [2][128]
   float* handed = reinterpret_cast<float*>(stat + 256);               // [128] (kShare) the reference after the last tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(handed + 128);
-  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_full = s_full + 2, *ref_set = p_full + 2 /* [2][4] */, *q_full = ref_set + 8, *q_empty = q_full + 1,
+  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2, *ref_set = p_full + 2 /* [2][4] */, *q_full = ref_set + 8, *q_empty = q_full + 1,
            *item_done = q_empty + 1, *sums_done = item_done + 1, *stat_full = sums_done + 1, *sums_free = stat_full + 1, *drain = sums_free + 1;
   unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this piece and the next
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
@@ -207,16 +213,17 @@ __global__ void __maxnreg__(152)
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 128);
+        mbar_init(&p_half[i], 4);
+        mbar_init(&p_full[i], 4);
         odd[i] = 0;
       }
       for (int i = 0; i < 8; ++i) mbar_init(&ref_set[i], 1);
-      mbar_init(q_full, 64);
+      mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       mbar_init(item_done, 1);
       mbar_init(sums_done, 1);
-      mbar_init(stat_full, 256);
-      mbar_init(sums_free, 256);
+      mbar_init(stat_full, 8);
+      mbar_init(sums_free, 8);
       mbar_init(drain, 1);
       *fail = 0;
       mbar_init_fence();
@@ -306,12 +313,16 @@ __global__ void __maxnreg__(152)
   // (384 threads of 152 registers at the start; the softmax warps take what the other four need not hold)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
-      // ============================================== copies: keys and values of the pieces, in the order in which they are used
-      const int box = min(a.c.page_size, kKeys);
+    if (warp == 8 || warp == 10) {
+      // ============================================== copies: keys (warp 8) and values (warp 10) of the pieces, in a ring that they fill in
+      // the order in which the products ask for them. One warp alone, some 600 cycles a tile, could not
+      // keep the memory busy with small pages.
       Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
       Piece p;
-      uint32_t rc = 0;
+      const bool is_k = warp == 8;
+      const CUtensorMap* map = is_k ? &map_k : &map_v;
+      const int box = min(a.c.page_size, kKeys);
+      uint32_t rc0 = 0, last = 0;
       bool ok = true;
       while (ok && walk.next(a, p)) {
         const int n = p.t1 - p.t0, end = walk.w.end;
@@ -321,23 +332,12 @@ __global__ void __maxnreg__(152)
           const int place = (p.t0 + j) * kKeys + lane * box;
           return j < n && lane * box < kKeys && place < end ? list[place >> a.c.page_shift] : 0;
         };
-        int id_before = 0, id = 0, id_next = page_of(0);
-        for (int e = 0; e < 2 * n; ++e) {
-          bool is_k;
-          int j;
-          if (MODE == kPair) {
-            is_k = !(e & 1);
-            j = e >> 1;
-          } else {
-            is_k = e == 0 || ((e & 1) && e != 2 * n - 1);
-            j = is_k ? (e + 1) >> 1 : e == 2 * n - 1 ? n - 1 : (e >> 1) - 1;
-          }
-          if (is_k) {
-            id_before = id;
-            id = id_next;
-            id_next = page_of(j + 1);
-          }
-          const int pg = is_k || MODE == kPair || e == 2 * n - 1 ? id : id_before;
+        int id_next = page_of(0);
+        for (int j = 0; j < n; ++j) {
+          const int id = id_next;
+          id_next = page_of(j + 1);
+          // (a key tile is asked for one step ahead of the value tile before it)
+          const uint32_t rc = rc0 + (MODE == kPair ? 2 * j + !is_k : is_k ? max(0, 2 * j - 1) : min(2 * j + 2, 2 * n - 1));
           const int slot = rc % kRing;
           if (!hold_warp(&empty[slot], ((rc / kRing) & 1u) ^ 1u, fail)) {
             ok = false;
@@ -345,24 +345,26 @@ __global__ void __maxnreg__(152)
           }
           const int place = (p.t0 + j) * kKeys, boxes = (min(kKeys, end - place) + box - 1) / box;
           if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * DIM * 2));
-          __syncwarp();
           if (lane < boxes) {
             int row = a.no_row;
-            if (pg >= 0 && pg < a.c.n_pages) row = pg * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
+            if (id >= 0 && id < a.c.n_pages) row = id * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
             else raise_status(a.c.status, ARCS_ERR_PAGE);
             const int y = a.by_row ? row : p.head, z = a.by_row ? 0 : row;
             char* dst = ring + slot * P::kTile + lane * box * 128;
 #pragma unroll
-            for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), is_k ? &map_k : &map_v, c * 64, y, z, &full[slot]);
+            for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), map, c * 64, y, z, &full[slot]);
           }
-          ++rc;
+          __syncwarp();
+          last = rc + 1;
         }
+        rc0 += 2 * n;
       }
       if (!ok && lane == 0)  // the copies in flight land before the CTA's memory goes to another
-        for (uint32_t i = rc > (uint32_t)kRing ? rc - kRing : 0; i < rc; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
+        for (uint32_t i = last > (uint32_t)kRing ? last - kRing : 0; i < last; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
     } else if (warp == 9) {
       // ============================================== products
-      if (lane == 0) {
+      {
+        const uint32_t on = elect_one();
         constexpr uint32_t kScores = mma_desc(128, kKeys, W::kBf16, false), kValues = mma_desc(128, DIM, W::kBf16, true);
         Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
         Piece p;
@@ -372,91 +374,98 @@ __global__ void __maxnreg__(152)
           const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2), ka = smem_addr(ring) + at * P::kTile;
 #pragma unroll
           for (int i = 0; i < DIM / 16; ++i)
-            mma_ss(tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
+            mma_ss(on, tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
                    i > 0);
         };
-        auto values = [&](int b, int sums, uint32_t at, bool first) {  // weights of score tile b x the values in ring slot `at`
+        // weights of score tile b x the values in ring slot `at`: the first half of the keys as soon as their
+        // weights are there
+        auto values = [&](int b, int sums, uint32_t at, bool first) {
           const uint32_t va = smem_addr(ring) + at * P::kTile;
 #pragma unroll
-          for (int i = 0; i < kKeys / 16; ++i)
-            mma_ts(tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
+          for (int h = 0; h < 2; ++h) {
+            if (!hold_warp(h ? &p_full[b] : &p_half[b], (turn >> b) & 1u, fail)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int i = h * kKeys / 32; i < (h + 1) * kKeys / 32; ++i)
+              mma_ts(on, tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
+          }
+          turn ^= 1u << b;
+          return true;
         };
+        auto commit = [&](uint64_t* bar) { mma_commit(on, bar); };
         while (ok && walk.next(a, p)) {
           const int n = p.t1 - p.t0;
           const bool two = MODE == kPair && walk.w.n * a.group - p.block * kRows > 128;
-          ok = hold(q_full, k & 1u, fail);
+          ok = hold_warp(q_full, k & 1u, fail);
           tc_fence_after();
           uint32_t k_at = 0, v_at = 0;
           for (int j = 0; ok && j <= n; ++j) {
             // (the sums of the piece before have been read: asked before the first product into them)
-            if (j == 1 && k > 0 && !(ok = hold(sums_free, (k - 1u) & 1u, fail))) break;
+            if (j == 1 && k > 0 && !(ok = hold_warp(sums_free, (k - 1u) & 1u, fail))) break;
             if (MODE == kPair) {
               if (j >= 1) {
                 v_at = rc % kRing;
-                ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[0], turn & 1u, fail);
+                ok = hold_warp(&full[v_at], (rc / kRing) & 1u, fail);
                 if (!ok) break;
-                turn ^= 1u;
                 ++rc;
-                tc_fence_after();
-                values(0, 0, v_at, j == 1);
-                if (!two) mma_commit(&empty[v_at]);
+              }
+              if (j < n) {  // (looked at before the weights are waited for, not between the two products)
+                k_at = rc % kRing;
+                ok = hold_warp(&full[k_at], (rc / kRing) & 1u, fail);
+                if (!ok) break;
+                ++rc;
+              }
+              if (j >= 1) {
+                ok = values(0, 0, v_at, j == 1);
+                if (!ok) break;
+                if (!two) commit(&empty[v_at]);
               }
               if (j < n) {
-                k_at = rc % kRing;
-                ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
-                if (!ok) break;
-                ++rc;
                 scores(0, 0, k_at);
-                mma_commit(&s_full[0]);
-                if (!two) mma_commit(&empty[k_at]);
-                if (!two && j == n - 1) mma_commit(q_empty);
+                commit(&s_full[0]);
+                if (!two) commit(&empty[k_at]);
+                if (!two && j == n - 1) commit(q_empty);
               }
               if (two && j >= 1) {
-                ok = hold(&p_full[1], (turn >> 1) & 1u, fail);
+                ok = values(1, 1, v_at, j == 1);
                 if (!ok) break;
-                turn ^= 2u;
-                tc_fence_after();
-                values(1, 1, v_at, j == 1);
-                mma_commit(&empty[v_at]);
+                commit(&empty[v_at]);
               }
               if (two && j < n) {
                 scores(1, 1, k_at);
-                mma_commit(&s_full[1]);
-                mma_commit(&empty[k_at]);
-                if (j == n - 1) mma_commit(q_empty);
+                commit(&s_full[1]);
+                commit(&empty[k_at]);
+                if (j == n - 1) commit(q_empty);
               }
             } else {
               if (j < n) {
                 k_at = rc % kRing;
-                ok = hold(&full[k_at], (rc / kRing) & 1u, fail);
+                ok = hold_warp(&full[k_at], (rc / kRing) & 1u, fail);
                 if (!ok) break;
                 ++rc;
                 scores(j & 1, 0, k_at);
-                mma_commit(&s_full[j & 1]);
-                mma_commit(&empty[k_at]);
-                if (j == n - 1) mma_commit(q_empty);
+                commit(&s_full[j & 1]);
+                commit(&empty[k_at]);
+                if (j == n - 1) commit(q_empty);
               }
               if (j >= 1) {
                 const int b = (j - 1) & 1;
                 v_at = rc % kRing;
-                ok = hold(&full[v_at], (rc / kRing) & 1u, fail) && hold(&p_full[b], (turn >> b) & 1u, fail);
+                ok = hold_warp(&full[v_at], (rc / kRing) & 1u, fail) && values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
                 if (!ok) break;
-                turn ^= 1u << b;
                 ++rc;
-                tc_fence_after();
-                values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
-                mma_commit(&empty[v_at]);
-                if (MODE == kShare) mma_commit(sums_done);
+                commit(&empty[v_at]);
+                if (MODE == kShare) commit(sums_done);
               }
             }
           }
           if (!ok) break;
-          mma_commit(item_done);
+          commit(item_done);
           ++k;
         }
         if (!ok) {
-          mma_commit(drain);
-          mbar_wait(drain, 0);
+          commit(drain);
+          if (lane == 0) mbar_wait(drain, 0);
         }
       }
       __syncwarp();
@@ -464,20 +473,19 @@ __global__ void __maxnreg__(152)
       // ============================================== queries of the next piece, once the products have done with those of this one
       Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
       Piece p;
-      const int at = tid - 320;
       uint32_t k = 0;
       while (walk.next(a, p)) {
         if (k > 0 && !hold_warp(q_empty, (k - 1u) & 1u, fail)) break;
         constexpr int kChunks = DIM / 8;
         const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
         const char* from = a.q + walk.w.off * a.q_token_stride;
-        for (int i = at; i < rows * kChunks; i += 64) {
+        for (int i = lane; i < rows * kChunks; i += 32) {
           const int r = i / kChunks, c = i % kChunks, x = p.block * kRows + r, node = x / a.group, h = p.head * a.group + x - node * a.group;
           copy16(sq + (r >> 7) * (128 * DIM * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), from + node * a.q_token_stride + h * a.q_head_stride + c * 16);
         }
         copy16_wait();
         fence_proxy_async();
-        mbar_arrive(q_full);
+        arrive_warp(q_full);
         ++k;
       }
     }
@@ -554,41 +562,37 @@ __global__ void __maxnreg__(152)
           const float now = moves ? most : before;
           if (MODE == kShare) {
             handed[row_t] = now;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ref_set[grp * 4 + (warp & 3)]);
+            arrive_warp(&ref_set[grp * 4 + (warp & 3)]);
           }
           if (__any_sync(0xFFFFFFFFu, now != m)) {
             l *= now != m ? exp2_approx(m - now) : 1.0f;
             m = now;
           }
-          if (__any_sync(0xFFFFFFFFu, moves)) {
-            const bool some = MODE == kSplit ? j >= 2 : j >= 1;  // (there is a sum to bring down)
-            if (some) {
-              if (MODE == kShare) {
-                if (!hold_warp(sums_done, (done + j - 1u) & 1u, fail)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
+          if (__any_sync(0xFFFFFFFFu, moves) && j >= (MODE == kSplit ? 2 : 1)) {  // there are sums to bring down
+            if (MODE == kShare) {
+              if (!hold_warp(sums_done, (done + j - 1u) & 1u, fail)) {
+                ok = false;
+                break;
               }
-              const float f = moves ? exp2_approx(before - now) : 1.0f;
-              const uint64_t f2 = pair_of(f, f);
-              const uint32_t sums = lanes + P::kSums + (MODE == kShare ? 0 : grp * DIM);
+              tc_fence_after();
+            }
+            const float f = moves ? exp2_approx(before - now) : 1.0f;
+            const uint64_t f2 = pair_of(f, f);
+            const uint32_t sums = lanes + P::kSums + (MODE == kShare ? 0 : grp * DIM);
 #pragma unroll 1
-              for (int i = 0; i < DIM / 32; ++i) {
-                uint32_t o[32];
-                tmem_ld32(o, sums + i * 32);
-                tmem_wait_ld();
-                tmem_use(o);
+            for (int i = 0; i < DIM / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld16(o, sums + i * 16);
+              tmem_wait_ld();
+              tmem_use(o);
 #pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                  float y0, y1;
-                  pair_out(mul_pair(pair_of(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), f2), y0, y1);
-                  o[c] = __float_as_uint(y0);
-                  o[c + 1] = __float_as_uint(y1);
-                }
-                tmem_st32(sums + i * 32, o);
+              for (int c = 0; c < 16; c += 2) {
+                float y0, y1;
+                pair_out(mul_pair(pair_of(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), f2), y0, y1);
+                o[c] = __float_as_uint(y0);
+                o[c + 1] = __float_as_uint(y1);
               }
+              tmem_st16(sums + i * 16, o);
             }
           }
           const float ref = W::kShift - (m == -INFINITY ? 0.0f : m);
@@ -607,11 +611,18 @@ __global__ void __maxnreg__(152)
               w[c >> 1] = W::pack(e0, e1);
             }
             tmem_st16(score + i * 16, w);
+            if (i == kKeys / 64 - 1 && !tail) {  // half of the weights are there
+              tmem_wait_st();
+              tc_fence_before();
+              arrive_warp(&p_half[grp]);
+            }
           }
           float l0, l1;
           pair_out(add_pair(sum[0], sum[1]), l0, l1);
           l += l0 + l1;
           tmem_wait_st();
+        } else if (!tail) {
+          arrive_warp(&p_half[grp]);
         }
         if (tail && (MODE != kPair || grp == 0)) {
           // Values behind the last node are whatever the page holds, and 0 times NaN is NaN: they become
@@ -646,7 +657,8 @@ __global__ void __maxnreg__(152)
           fence_proxy_async();
         }
         tc_fence_before();
-        mbar_arrive(&p_full[grp]);
+        if (tail) arrive_warp(&p_half[grp]);
+        arrive_warp(&p_full[grp]);
       }
       if (!ok) break;
 
@@ -657,7 +669,7 @@ __global__ void __maxnreg__(152)
       }
       tc_fence_after();
       if (MODE != kPair) stat[grp * 128 + row_t] = make_float2(m, l);
-      mbar_arrive(stat_full);
+      arrive_warp(stat_full);
       if (!hold_warp(stat_full, k & 1u, fail)) {
         ok = false;
         break;
@@ -682,7 +694,7 @@ __global__ void __maxnreg__(152)
           if (!whole) a.part_stat[block] = make_float2(m - W::kShift, l);
           else if (a.lse) a.lse[(int64_t)(off + node) * a.Hq + head_q] = sees ? (m - W::kShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
         }
-#pragma unroll 1
+#pragma unroll 2
         for (int i = 0; i < kCols / 32; ++i) {
           const int col = c0 + i * 32;
           uint32_t o[32];
@@ -731,7 +743,7 @@ __global__ void __maxnreg__(152)
       }
       if (tid == 0) odd[(k + 1) & 1u] = 0;
       tc_fence_before();
-      mbar_arrive(sums_free);
+      arrive_warp(sums_free);
       rc0 += 2 * n;
       done += n;
       if (MODE == kShare && warp_live && (n & 1) == grp && n > grp) ++set;  // (the piece's last tile was the other group's: nobody asked for its reference)
