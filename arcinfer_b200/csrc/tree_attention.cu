@@ -122,9 +122,10 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a,
   if (e != cudaSuccess) return set_error(ARCS_ERR_CUDA, cudaGetErrorString(e));
   tree_tiles_kernel<T, DIM, MODE><<<kCtas, kTileThreads, P::kSmem, st>>>(mk, mv, a);
   if (int rc = check_launch("tree_attention")) return rc;
-  const int64_t rows = (int64_t)a.T * a.Hq;
-  if (rows <= 1024) launch_behind(join_kernel<T, DIM, MODE, 4>, dim3((unsigned)rows), dim3(kJoinThreads), 0, st, a, kCtas);
-  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(kJoinThreads), 0, st, a, kCtas);
+  const int blocks = (a.max_nodes * a.group + P::kRows - 1) / P::kRows;
+  const int64_t items = (int64_t)a.c.slots * a.c.heads * blocks;
+  if (items <= kCtas / 2) launch_behind(join_kernel<T, DIM, MODE, 4>, dim3((unsigned)items, (unsigned)a.part_rows), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
+  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3(kCtas - 1, (unsigned)(a.part_rows + 15) / 16), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
   return check_launch("tree_attention");
 }
 

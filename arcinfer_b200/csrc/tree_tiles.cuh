@@ -755,110 +755,166 @@ __global__ void __maxnreg__(152)
   if (warp == 9) tmem_free(tmem, 512);
 }
 
-// The pieces of items that were cut, joined. A CTA of four warps takes a row (WARPS = 4: there are few, and
-// each may have a hundred pieces) or four; a warp asks for four pieces' sums at a time, weights beside
-// them. Small enough (56 registers, 128 threads) to be on the SM, its way found, while the last pieces are
-// still worked on.
+// Where unit u lies: its slot, and the units before that. Asked by a whole warp; up to 128 slots it adds
+// them up itself (`total` too), else it searches the running sum that tree_tiles_kernel left.
+template <int KEYS, int ROWS>
+__device__ __forceinline__ uint32_t add_up(const TreeDev& a, uint32_t (&before)[4], uint32_t (&own)[4]) {
+  const int lane = threadIdx.x & 31;
+  uint32_t total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    own[i] = 0;
+    if (i * 32 + lane < a.c.slots) own[i] = (uint32_t)slot_work<KEYS, ROWS>(a, i * 32 + lane).units;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t x = own[i];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      if (lane >= o) x += y;
+    }
+    before[i] = total + x - own[i];
+    total += __shfl_sync(0xFFFFFFFFu, x, 31);
+  }
+  return total;
+}
+
+// The pieces of items that were cut, joined. WARPS = 4, for few items of maybe a hundred pieces each:
+// blockIdx.x is the item (slot, key head, block), and four warps work on one row. WARPS = 1, for many:
+// every item that is cut begins in one CTA and goes on in the next, so blockIdx.x names the CTA in
+// which it begins, and a warp takes a row. A warp asks for some pieces' sums at a time, their statistics
+// beside them. Small enough (56 registers, 128 threads) to be on the SM, its way found, while the last
+// pieces are still worked on.
 constexpr int kJoinThreads = 128;
 template <typename T, int DIM, int MODE, int WARPS>
-__global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, int ctas, int blocks) {
   using P = TilePlan<DIM, MODE>;
   using W = Weight<T>;
   constexpr int kPer = DIM / 32;
   __shared__ float2 s_stat[4];
   __shared__ float s_sum[WARPS == 4 ? 4 : 1][WARPS == 4 ? DIM : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = WARPS == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + warp;
-  const int t = (int)(row / a.Hq), h = (int)(row % a.Hq);
-  const int s = t < a.T ? slot_of_row(a.node_off, a.c.slots, t) : -1;
-  SlotWork w;
-  w.n = 0;
-  if (s >= 0) w = slot_work<P::kKeys, P::kRows>(a, s);
-  if (w.n == 0) return;
-  const int head = h / a.group, r = (t - w.off) * a.group + h % a.group, block = r / P::kRows, rr = r % P::kRows;
-  uint32_t total = 0, before = 0;
-  if (a.c.slots <= 128) {
-    for (int i = lane; i < a.c.slots; i += 32) {
-      const uint32_t u = (uint32_t)slot_work<P::kKeys, P::kRows>(a, i).units;
-      total += u;
-      if (i < s) before += u;
+  uint32_t total = 0, base = 0, u = 0;
+  int s = WARPS == 4 ? (int)blockIdx.x / (a.c.heads * blocks) : -1;
+  const bool few = WARPS == 4 || a.c.slots <= 128;  // (few items are of few slots)
+  if (few) {
+    uint32_t before[4], own[4];
+    total = add_up<P::kKeys, P::kRows>(a, before, own);
+    u = first_unit(total, (int)blockIdx.x + 1, ctas);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool mine = WARPS == 4 ? i * 32 + lane == s : before[i] <= u && u < before[i] + own[i];
+      const unsigned hit = __ballot_sync(0xFFFFFFFFu, mine);
+      if (hit) {
+        s = i * 32 + __ffs((int)hit) - 1;
+        base = __shfl_sync(0xFFFFFFFFu, before[i], __ffs((int)hit) - 1);
+      }
     }
-    total = __reduce_add_sync(0xFFFFFFFFu, total);
-    before = __reduce_add_sync(0xFFFFFFFFu, before);
-    pdl_wait();
   } else {
     pdl_wait();
     total = __ldcg(a.prefix + a.c.slots);
-    before = __ldcg(a.prefix + s);
-  }
-  const uint32_t u = before + (uint32_t)((head * w.blocks + block) * w.tiles);
-  const int c0 = cta_of_unit(total, u, ctas), c1 = cta_of_unit(total, u + (uint32_t)w.tiles - 1u, ctas);
-  if (c0 == c1) return;
-  float m = -INFINITY, l = 0.0f, o[kPer];
-#pragma unroll
-  for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
-  constexpr int kAtOnce = DIM == 256 ? 2 : 4;
-  for (int b = c0 + (WARPS == 4 ? warp : 0) * kAtOnce; b <= c1; b += kAtOnce * WARPS) {
-    float y[kAtOnce][kPer];
-    float2 st[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int c = b + i;
-      // (with fewer units than CTAs some of them have none)
-      const bool there = c <= c1 && first_unit(total, c, ctas) != first_unit(total, c + 1, ctas);
-      const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
-      st[i] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
-      if (there) {
-        const float* src = a.part + at * DIM + lane * kPer;
-        st[i] = __ldcg(a.part_stat + at);
-        if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src));
-#pragma unroll
-        for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
-      }
+    u = first_unit(total, (int)blockIdx.x + 1, ctas);
+    int lo = 0, n = a.c.slots;  // the last slot with prefix <= u (those without units share theirs with the next)
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = lo + lane * step;
+      const unsigned b = __ballot_sync(0xFFFFFFFFu, at < lo + n && __ldcg(a.prefix + at) <= u);
+      const int j = b ? 31 - __clz(b) : 0;
+      n = min(step, lo + n - (lo + j * step));
+      lo += j * step;
     }
-    float top = m;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
-    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
-    m = top;
-    l = weighed(f, l);
-#pragma unroll
-    for (int d = 0; d < kPer; ++d) o[d] = weighed(f, o[d]);
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const float wt = exp2_approx(st[i].x - ref);
-      l += wt * st[i].y;
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, y[i][d]);
-    }
+    s = lo;
+    base = __ldcg(a.prefix + s);
   }
-  if (WARPS == 4) {  // the four warps' shares: a quarter of the row each
-    if (lane == 0) s_stat[warp] = make_float2(m, l);
-#pragma unroll
-    for (int d = 0; d < kPer; ++d) s_sum[warp][lane * kPer + d] = o[d];
-    __syncthreads();
-    m = fmaxf(fmaxf(s_stat[0].x, s_stat[1].x), fmaxf(s_stat[2].x, s_stat[3].x));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
+  if (s < 0 || (WARPS == 1 && u >= total)) return;
+  const SlotWork w = slot_work<P::kKeys, P::kRows>(a, s);
+  if (w.n == 0) return;
+  int head, block;
+  if (WARPS == 4) {
+    const int x = (int)blockIdx.x - s * a.c.heads * blocks;
+    head = x / blocks;
+    block = x - head * blocks;
+    if (block >= w.blocks) return;
+  } else {
+    const int x = (int)(u - base) / w.tiles;
+    head = x / w.blocks;
+    block = x - head * w.blocks;
+  }
+  const uint32_t begins = base + (uint32_t)((head * w.blocks + block) * w.tiles);
+  const int c0 = cta_of_unit(total, begins, ctas), c1 = cta_of_unit(total, begins + (uint32_t)w.tiles - 1u, ctas);
+  if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return;  // not cut, or cut before
+  const int rows = min(P::kRows, w.n * a.group - block * P::kRows);
+  if (few) pdl_wait();
+  for (int rr = (int)blockIdx.y * (4 / WARPS) + (WARPS == 4 ? 0 : warp); rr < rows; rr += (int)gridDim.y * (4 / WARPS)) {
+    float m = -INFINITY, l = 0.0f, o[kPer];
 #pragma unroll
     for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
-    if (warp != 0) return;
+    constexpr int kAtOnce = DIM == 256 ? 2 : 4;
+    for (int b = c0 + (WARPS == 4 ? warp : 0) * kAtOnce; b <= c1; b += kAtOnce * WARPS) {
+      float y[kAtOnce][kPer];
+      float2 st[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float wt = exp2_approx(s_stat[i].x - ref);
-      l += weighed(wt, s_stat[i].y);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int c = b + i;
+        // (with fewer units than CTAs some of them have none)
+        const bool there = c <= c1 && (total >= (uint32_t)ctas || first_unit(total, c, ctas) != first_unit(total, c + 1, ctas));
+        const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
+        st[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, s_sum[i][lane * kPer + d]);
+        for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
+        if (there) {
+          const float* src = a.part + at * DIM + lane * kPer;
+          st[i] = __ldcg(a.part_stat + at);
+          if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+#pragma unroll
+          for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
+      const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+      m = top;
+      l = weighed(f, l);
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) o[d] = weighed(f, o[d]);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float wt = exp2_approx(st[i].x - ref);
+        l += wt * st[i].y;
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, y[i][d]);
+      }
+    }
+    if (WARPS == 4) {  // the four warps' shares
+      if (lane == 0) s_stat[warp] = make_float2(m, l);
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) s_sum[warp][lane * kPer + d] = o[d];
+      __syncthreads();
+      m = fmaxf(fmaxf(s_stat[0].x, s_stat[1].x), fmaxf(s_stat[2].x, s_stat[3].x));
+      const float ref = m == -INFINITY ? 0.0f : m;
+      l = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float wt = exp2_approx(s_stat[i].x - ref);
+        l += weighed(wt, s_stat[i].y);
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, s_sum[i][lane * kPer + d]);
+      }
+      __syncthreads();
+    }
+    if (WARPS == 1 || warp == 0) {
+      const bool sees = l > 0.0f || l != l;
+      const float inv = sees ? 1.0f / l : 0.0f;
+      const int x = block * P::kRows + rr, node = x / a.group, h = head * a.group + x - node * a.group;
+      char* dst = a.out + (w.off + node) * a.out_token_stride + h * a.out_head_stride + lane * kPer * 2;
+#pragma unroll
+      for (int d = 0; d < kPer; d += 2) *reinterpret_cast<uint32_t*>(dst + d * 2) = sees ? W::pack(o[d] * inv, o[d + 1] * inv) : 0u;
+      if (a.lse && lane == 0) a.lse[(int64_t)(w.off + node) * a.Hq + h] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
   }
-  const bool sees = l > 0.0f || l != l;
-  const float inv = sees ? 1.0f / l : 0.0f;
-  char* dst = a.out + t * a.out_token_stride + h * a.out_head_stride + lane * kPer * 2;
-#pragma unroll
-  for (int d = 0; d < kPer; d += 2) *reinterpret_cast<uint32_t*>(dst + d * 2) = sees ? W::pack(o[d] * inv, o[d + 1] * inv) : 0u;
-  if (a.lse && lane == 0) a.lse[(int64_t)t * a.Hq + h] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 }  // namespace arcs
