@@ -110,7 +110,6 @@ bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const Row
 
 constexpr int kCtas = kSmCount;
 int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair : kSplit; }
-int keys_of(int dim, int mode) { return dim == 256 ? 64 : 128; }
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -135,7 +134,7 @@ extern "C" size_t arcs_tree_attention_workspace_bytes(int32_t slots, int32_t hea
   if (slots < 1 || heads < 1 || Hq < heads || Hq % heads || Hq / heads > 64 || (dim != 64 && dim != 128 && dim != 256) || max_nodes < 1 || max_nodes > ARCS_TREE_MAX) return 0;
   const int rows = max_nodes * (Hq / heads), most = rows_of(mode_of(dim, rows));
   const size_t blocks = (size_t)kCtas * 2 * (rows < most ? rows : most);
-  return round16(((size_t)slots + 1) * 4) + round16(blocks * 8) + blocks * dim * 4;
+  return round16(((size_t)slots + 2) * 4) + round16(blocks * 8) + blocks * dim * 4;
 }
 
 extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stream) {
@@ -180,12 +179,12 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
 
   RowPlan r;
   if (plan_rows(c, &r)) {
-    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = keys_of(c->dim, mode);
-    if ((((int64_t)c->max_pages * c->page_size + keys - 1) / keys) * c->slots * c->heads * ((rows + most - 1) / most) > 0x7FFFFFFFll)
+    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = 128, part = c->dim == 256 ? 64 : 128;  // (as in TilePlan)
+    if ((((int64_t)c->max_pages * c->page_size + keys - 1) / keys) * c->slots * c->heads * ((rows + most - 1) / most) > 0x0FFFFFFFll)
       return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
     if (!encode_tiled()) return set_error(ARCS_ERR_CUDA, "tree_attention: the driver makes no tensor maps");
     CUtensorMap mk, mv;
-    if (!make_map(&mk, c, a.c.k, r, keys) || !make_map(&mv, c, a.c.v, r, keys)) return set_error(ARCS_ERR_CUDA, "tree_attention: no tensor map for these pools");
+    if (!make_map(&mk, c, a.c.k, r, keys) || !make_map(&mv, c, a.c.v, r, part)) return set_error(ARCS_ERR_CUDA, "tree_attention: no tensor map for these pools");
     a.by_row = r.by_row;
     a.page_rows = (int32_t)r.page_rows;
     a.head_rows = (int32_t)r.head_rows;
@@ -194,8 +193,8 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
     char* ws = static_cast<char*>(g->workspace);
     const size_t blocks = (size_t)kCtas * 2 * a.part_rows;
     a.prefix = reinterpret_cast<uint32_t*>(ws);
-    a.part_stat = reinterpret_cast<float2*>(ws + round16(((size_t)c->slots + 1) * 4));
-    a.part = reinterpret_cast<float*>(ws + round16(((size_t)c->slots + 1) * 4) + round16(blocks * 8));
+    a.part_stat = reinterpret_cast<float2*>(ws + round16(((size_t)c->slots + 2) * 4));
+    a.part = reinterpret_cast<float*>(ws + round16(((size_t)c->slots + 2) * 4) + round16(blocks * 8));
 #define ARCS_LAUNCH(TYPE)                                                                \
   do {                                                                                   \
     if (c->dim == 256) return launch_tiles<TYPE, 256, kShare>(mk, mv, a, st);           \

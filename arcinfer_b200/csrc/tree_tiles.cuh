@@ -32,16 +32,23 @@ enum { kSplit = 0, kPair = 1, kShare = 2 };
 
 template <int DIM, int MODE>
 struct TilePlan {
-  static constexpr int kKeys = DIM == 256 ? 64 : 128;
+  static constexpr int kKeys = 128;                            // keys in a tile
   static constexpr int kRows = MODE == kPair ? 256 : 128;      // rows of an item
+  // Pieces of a tile in the ring: at dim 256 the keys come as two halves of 128 values each, the values as
+  // two halves of 64 keys. (Tiles of 64 keys instead cost a third more: a product of 128 x 64 x 16 takes
+  // 56 cycles, not the half of 64, because the queries are read again for every one.)
+  static constexpr int kSub = DIM == 256 ? 2 : 1;
   static constexpr int kQBytes = kRows * DIM * 2;
-  static constexpr int kTile = kKeys * DIM * 2;
-  // tiles in the ring: 160 KB a CTA keep the memory busy (20 MB under way on all of them). kSplit and
-  // kShare leave room beside them for a CTA of join_kernel.
-  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : MODE == kSplit ? 5 : 5;
+  static constexpr int kTile = kKeys * DIM * 2 / kSub;         // 32 KB, at dim 64 16 KB
+  // slots of the ring: 128 to 160 KB a CTA keep the memory busy (20 MB under way on all of them). kSplit
+  // and kShare leave room beside them for a CTA of join_kernel.
+  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : 5;
   static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 1024;
   static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
   static constexpr uint32_t kSums = 256;
+  // What a tile of keys costs: 3 for two tiles of rows, 2 where an item has only one of its two; and an
+  // item for its beginning and end, about as much as two tiles.
+  static constexpr int kCost = MODE == kPair ? 3 : 1, kCostOne = MODE == kPair ? 2 : 1, kItemCost = 2 * kCost;
 };
 static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kShare>::kSmem <= 232448 &&
               TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
@@ -49,10 +56,15 @@ static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kS
 constexpr int kTileThreads = 384;
 
 struct SlotWork {
-  int off, n, len, end, tiles, blocks, units;  // blocks of rows a key head; units: tiles of keys x blocks x key heads
+  int off, n, len, tiles, blocks;  // rows of the step, nodes, settled tokens; tiles of keys, blocks of rows a key head
   bool bad;
 };
-template <int KEYS, int ROWS>
+template <typename P>
+__device__ __forceinline__ void size_up(const TreeDev& a, SlotWork& w) {
+  w.tiles = w.n > 0 ? (w.len + w.n + P::kKeys - 1) / P::kKeys : 0;
+  w.blocks = w.n > 0 ? (w.n * a.group + P::kRows - 1) / P::kRows : 0;
+}
+template <typename P>
 __device__ __forceinline__ SlotWork slot_work(const TreeDev& a, int s) {
   SlotWork w;
   const int r1 = a.node_off[s + 1], used = a.c.used[s];
@@ -61,46 +73,72 @@ __device__ __forceinline__ SlotWork slot_work(const TreeDev& a, int s) {
   w.len = a.c.len[s];
   w.bad = w.off < 0 || r1 < w.off || r1 > a.T || w.n > a.max_nodes ||
           (w.n > 0 && (w.len < 0 || used < 0 || used > a.c.max_pages || (int64_t)w.len + w.n > ((int64_t)used << a.c.page_shift)));
-  if (w.bad || w.n == 0) {
-    w.n = w.end = w.tiles = w.blocks = w.units = 0;
-    return w;
-  }
-  w.end = w.len + w.n;
-  w.tiles = (w.end + KEYS - 1) / KEYS;
-  w.blocks = (w.n * a.group + ROWS - 1) / ROWS;
-  w.units = w.tiles * w.blocks * a.c.heads;
+  if (w.bad) w.n = 0;
+  size_up<P>(a, w);
   return w;
 }
 
-// All slots' units in a row (slot, key head, block of rows, tile of keys) are dealt out evenly: CTA c of G takes
-// [total c / G, total (c + 1) / G), so the lengths need not be known on the host. An item that lies in
-// one CTA is finished there; one that is cut leaves partial results, joined by join_kernel.
+// The work is dealt out evenly in units of cost: all slots' items (key head, block of rows) lie in a row,
+// each `extra` units for itself and then its tiles; CTA c of G takes what begins in [total c / G,
+// total (c + 1) / G), so the lengths need not be known on the host. An item that lies in one CTA is
+// finished there; one that is cut leaves partial results, joined by join_kernel. `extra` is zero where a CTA
+// gets fewer than 16 tiles: there an even share of tiles counts for more.
+template <typename P>
+struct Costs {
+  int first, head, last;  // units of an item with all its rows, of a key head's items; of a tile in the head's last item
+  __device__ __forceinline__ Costs(const TreeDev& a, const SlotWork& w, int extra) {
+    last = w.n * a.group - (w.blocks - 1) * P::kRows <= 128 ? P::kCostOne : P::kCost;
+    first = w.tiles * P::kCost + extra;
+    head = w.blocks > 0 ? (w.blocks - 1) * first + w.tiles * last + extra : 0;
+  }
+};
 __device__ __forceinline__ uint32_t first_unit(uint32_t total, int c, int ctas) { return (uint32_t)((uint64_t)total * (uint32_t)c / (uint32_t)ctas); }
 __device__ __forceinline__ int cta_of_unit(uint32_t total, uint32_t u, int ctas) { return (int)(((uint64_t)(u + 1) * (uint32_t)ctas - 1) / total); }
+template <typename P>
+__device__ __forceinline__ int extra_units(uint32_t plain_total, int ctas) { return plain_total >= 16u * P::kCost * (uint32_t)ctas ? P::kItemCost : 0; }
+
+struct Place {  // of an item
+  int head, block, cost;
+  uint32_t begins;  // its first unit
+};
+// the item that unit x of a slot belongs to
+template <typename P>
+__device__ __forceinline__ Place place_of(const SlotWork& w, const Costs<P>& c, uint32_t base, int x) {
+  Place p;
+  p.head = x / c.head;
+  const int y = x - p.head * c.head;
+  p.block = min(y / c.first, w.blocks - 1);
+  p.cost = p.block == w.blocks - 1 ? c.last : P::kCost;
+  p.begins = base + (uint32_t)(p.head * c.head + p.block * c.first);
+  return p;
+}
 
 struct Piece {  // of an item: tiles [t0, t1)
   int head, block, t0, t1;
 };
-template <int KEYS, int ROWS>
+template <typename P>
 struct Walk {
   uint32_t u, u1, base;
-  int s;
+  int s, extra;
   SlotWork w;
-  __device__ __forceinline__ Walk(const TreeDev& a, uint32_t u0_, uint32_t u1_, int s0, uint32_t base0) : u(u0_), u1(u1_), base(base0), s(s0), w(slot_work<KEYS, ROWS>(a, s0)) {}
   __device__ __forceinline__ bool next(const TreeDev& a, Piece& p) {
-    if (u >= u1) return false;
-    while (u >= base + (uint32_t)w.units) {
-      base += (uint32_t)w.units;
-      ++s;
-      w = slot_work<KEYS, ROWS>(a, s);
+    while (u < u1) {
+      Costs<P> c(a, w, extra);
+      while (u >= base + (uint32_t)(c.head * a.c.heads)) {
+        base += (uint32_t)(c.head * a.c.heads);
+        w = slot_work<P>(a, ++s);
+        c = Costs<P>(a, w, extra);
+      }
+      const Place at = place_of<P>(w, c, base, (int)(u - base));
+      const int from = (int)(u - at.begins) - extra, ends = w.tiles * at.cost, to = min((int)(u1 - at.begins) - extra, ends);
+      p.head = at.head;
+      p.block = at.block;
+      p.t0 = from <= 0 ? 0 : (from + at.cost - 1) / at.cost;
+      p.t1 = to <= 0 ? 0 : (to + at.cost - 1) / at.cost;
+      u = at.begins + (uint32_t)(to + extra);
+      if (p.t0 < p.t1) return true;
     }
-    const int x = (int)(u - base), item = x / w.tiles;
-    p.head = item / w.blocks;
-    p.block = item - p.head * w.blocks;
-    p.t0 = x - item * w.tiles;
-    p.t1 = min(w.tiles, p.t0 + (int)(u1 - u));
-    u += (uint32_t)(p.t1 - p.t0);
-    return true;
+    return false;
   }
 };
 
@@ -133,6 +171,21 @@ __device__ __forceinline__ void arrive_warp(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// The rows of an item to shared memory, swizzled as the tiles of keys are: thread `at` of `by`.
+template <int DIM, int ROWS>
+__device__ __forceinline__ void bring_queries(const TreeDev& a, const SlotWork& w, const Piece& p, char* sq, int at, int by) {
+  constexpr int kChunks = DIM / 8;
+  const int rows = min(ROWS, w.n * a.group - p.block * ROWS), c = at % kChunks, step = by / kChunks;
+  int r = at / kChunks;
+  const int x = p.block * ROWS + r;
+  int node = x / a.group, g = x - node * a.group;
+  const char* from = a.q + (int64_t)w.off * a.q_token_stride + (int64_t)(p.head * a.group) * a.q_head_stride + c * 16;
+  for (; r < rows; r += step) {
+    copy16(sq + (r >> 7) * (128 * DIM * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), from + node * a.q_token_stride + g * a.q_head_stride);
+    for (g += step; g >= a.group; g -= a.group) ++node;
+  }
+}
+
 template <typename T> struct Weight;
 template <> struct Weight<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
@@ -163,6 +216,38 @@ template <> struct Weight<__half> {
 // weight * sum, where the weight may have been rounded to nothing and the sum may be infinite
 __device__ __forceinline__ float weighed(float w, float o) { return w == 0.0f ? (fabsf(o) <= 3.402823466e38f ? 0.0f : o) : w * o; }
 
+// Up to 128 slots, a warp on its own: four slots a lane, the units before each, and the units in all.
+template <typename P>
+__device__ __forceinline__ uint32_t add_up(const TreeDev& a, int ctas, SlotWork (&w)[4], uint32_t (&before)[4], uint32_t (&own)[4], int& extra) {
+  const int lane = threadIdx.x & 31;
+  uint32_t plain = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i].n = 0;
+    w[i].bad = false;
+    if (i * 32 + lane < a.c.slots) w[i] = slot_work<P>(a, i * 32 + lane);
+    else size_up<P>(a, w[i]);
+    plain += (uint32_t)(Costs<P>(a, w[i], 0).head * a.c.heads);
+  }
+  extra = extra_units<P>(__reduce_add_sync(0xFFFFFFFFu, plain), ctas);
+  uint32_t total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    before[i] = own[i] = 0;
+    if (i * 32 >= a.c.slots) continue;
+    own[i] = (uint32_t)(Costs<P>(a, w[i], extra).head * a.c.heads);
+    uint32_t x = own[i];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      if (lane >= o) x += y;
+    }
+    before[i] = total + x - own[i];
+    total += __shfl_sync(0xFFFFFFFFu, x, 31);
+  }
+  return total;
+}
+
 template <typename T, int DIM, int MODE>
 __global__ void __maxnreg__(152)
     tree_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeDev a) {
@@ -175,7 +260,7 @@ __global__ void __maxnreg__(152)
   float2* stat = reinterpret_cast<float2*>(ring + kRing * P::kTile);  // [2][128]
   float* handed = reinterpret_cast<float*>(stat + 256);               // [128] (kShare) the reference after the last tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(handed + 128);
-  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2, *ref_set = p_full + 2 /* [2][4] */, *q_full = ref_set + 8, *q_empty = q_full + 1,
+  uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2, *ref_set = p_full + 2 /* [2][4] */, *q_first = ref_set + 8, *q_full = q_first + 1, *q_empty = q_full + 1,
            *item_done = q_empty + 1, *sums_done = item_done + 1, *stat_full = sums_done + 1, *sums_free = stat_full + 1, *drain = sums_free + 1;
   unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this piece and the next
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
@@ -191,19 +276,9 @@ __global__ void __maxnreg__(152)
 
   // ---- where this CTA's units begin. Up to 128 slots every warp adds up on its own, which asks for no
   // barrier but the one behind the set-up; more are added up by the whole CTA, in the ring's memory.
-  uint32_t total = 0, u0 = 0, u1 = 0, base = 0;
-  int s_first = -1;
+  Walk<P> walk;
+  uint32_t total = 0;
   const bool few = a.c.slots <= 128;
-  uint32_t own[4] = {0, 0, 0, 0};
-  if (few) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i * 32 < a.c.slots && i * 32 + lane < a.c.slots) {
-        const SlotWork w = slot_work<kKeys, kRows>(a, i * 32 + lane);
-        if (w.bad && cta == 0 && warp == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
-        own[i] = (uint32_t)w.units;
-      }
-  }
   if (warp == 9) {
     tmem_alloc(s_tmem, 512);
     if (lane == 0) {
@@ -218,6 +293,7 @@ __global__ void __maxnreg__(152)
         odd[i] = 0;
       }
       for (int i = 0; i < 8; ++i) mbar_init(&ref_set[i], 1);
+      mbar_init(q_first, 8);
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       mbar_init(item_done, 1);
@@ -228,70 +304,73 @@ __global__ void __maxnreg__(152)
       *fail = 0;
       mbar_init_fence();
     }
+    __syncwarp();
   }
+  walk.s = -1;
   if (few) {
-    uint32_t before[4];
+    SlotWork w[4];
+    uint32_t before[4], own[4];
+    total = add_up<P>(a, ctas, w, before, own, walk.extra);
+    walk.u = first_unit(total, cta, ctas);
+    walk.u1 = first_unit(total, cta + 1, ctas);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i * 32 >= a.c.slots) break;
-      uint32_t x = own[i];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-        if (lane >= o) x += y;
-      }
-      before[i] = total + x - own[i];
-      total += __shfl_sync(0xFFFFFFFFu, x, 31);
-    }
-    u0 = first_unit(total, cta, ctas);
-    u1 = first_unit(total, cta + 1, ctas);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i * 32 >= a.c.slots) break;
-      const unsigned hit = __ballot_sync(0xFFFFFFFFu, before[i] <= u0 && u0 < before[i] + own[i]);
+      const unsigned hit = __ballot_sync(0xFFFFFFFFu, before[i] <= walk.u && walk.u < before[i] + own[i]);
       if (hit) {
-        s_first = i * 32 + __ffs((int)hit) - 1;
-        base = __shfl_sync(0xFFFFFFFFu, before[i], __ffs((int)hit) - 1);
+        const int from = __ffs((int)hit) - 1;
+        walk.s = i * 32 + from;
+        walk.base = __shfl_sync(0xFFFFFFFFu, before[i], from);
+        walk.w.off = __shfl_sync(0xFFFFFFFFu, w[i].off, from);
+        walk.w.n = __shfl_sync(0xFFFFFFFFu, w[i].n, from);
+        walk.w.len = __shfl_sync(0xFFFFFFFFu, w[i].len, from);
       }
-      if (cta == 0 && warp == 0 && i * 32 + lane < a.c.slots) a.prefix[i * 32 + lane] = before[i];
+      if (w[i].bad && cta == 0 && warp == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
     }
-    if (cta == 0 && tid == 0) a.prefix[a.c.slots] = total;
+    size_up<P>(a, walk.w);
   } else {
     uint32_t* pre = reinterpret_cast<uint32_t*>(ring);
-    for (int s0 = 0; s0 < a.c.slots; s0 += kNT) {
-      const int s = s0 + tid;
-      uint32_t mine = 0;
-      if (s < a.c.slots) {
-        const SlotWork w = slot_work<kKeys, kRows>(a, s);
-        if (w.bad && cta == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
-        mine = (uint32_t)w.units;
-      }
-      uint32_t x = mine;
+    walk.extra = 0;
+    for (int turn = 0; turn < 2; ++turn) {  // the plain total first, which decides `extra`
+      total = 0;
+      for (int s0 = 0; s0 < a.c.slots; s0 += kNT) {
+        const int s = s0 + tid;
+        uint32_t mine = 0;
+        if (s < a.c.slots) {
+          const SlotWork w = slot_work<P>(a, s);
+          if (w.bad && cta == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
+          mine = (uint32_t)(Costs<P>(a, w, walk.extra).head * a.c.heads);
+        }
+        uint32_t x = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-        if (lane >= o) x += y;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (lane == 31) s_sums[warp] = x;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+        for (int i = 0; i < kNT / 32; ++i) {
+          const uint32_t v = s_sums[i];
+          if (i < warp) before += v;
+          all += v;
+        }
+        if (s < a.c.slots) pre[s] = total + before + x - mine;
+        total += all;
+        __syncthreads();
       }
-      if (lane == 31) s_sums[warp] = x;
-      __syncthreads();
-      uint32_t before = 0, all = 0;
-      for (int i = 0; i < kNT / 32; ++i) {
-        const uint32_t v = s_sums[i];
-        if (i < warp) before += v;
-        all += v;
-      }
-      if (s < a.c.slots) pre[s] = total + before + x - mine;
-      total += all;
-      __syncthreads();
+      if (turn == 0) walk.extra = extra_units<P>(total, ctas);
     }
     if (tid == 0) pre[a.c.slots] = total;
     __syncthreads();
-    if (cta == 0)
+    if (cta == 0) {
       for (int s = tid; s <= a.c.slots; s += kNT) a.prefix[s] = pre[s];
-    u0 = first_unit(total, cta, ctas);
-    u1 = first_unit(total, cta + 1, ctas);
+      if (tid == 0) a.prefix[a.c.slots + 1] = (uint32_t)walk.extra;
+    }
+    walk.u = first_unit(total, cta, ctas);
+    walk.u1 = first_unit(total, cta + 1, ctas);
     for (int s = tid; s < a.c.slots; s += kNT)
-      if (pre[s] <= u0 && u0 < pre[s + 1]) {
+      if (pre[s] <= walk.u && walk.u < pre[s + 1]) {
         s_begin[0] = (uint32_t)s;
         s_begin[1] = pre[s];
       }
@@ -301,14 +380,16 @@ __global__ void __maxnreg__(152)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  if (!few) {
-    s_first = (int)s_begin[0];
-    base = s_begin[1];
-  }
-  if (u0 == u1) {  // nothing for this CTA
+  if (walk.u == walk.u1) {  // nothing for this CTA
     if (warp == 9) tmem_free(tmem, 512);
     return;
   }
+  if (!few) {
+    walk.s = (int)s_begin[0];
+    walk.base = s_begin[1];
+    walk.w = slot_work<P>(a, walk.s);
+  }
+  Piece p;
 
   // (384 threads of 152 registers at the start; the softmax warps take what the other four need not hold)
   if (warp >= 8) {
@@ -317,47 +398,55 @@ __global__ void __maxnreg__(152)
       // ============================================== copies: keys (warp 8) and values (warp 10) of the pieces, in a ring that they fill in
       // the order in which the products ask for them. One warp alone, some 600 cycles a tile, could not
       // keep the memory busy with small pages.
-      Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
-      Piece p;
       const bool is_k = warp == 8;
       const CUtensorMap* map = is_k ? &map_k : &map_v;
-      const int box = min(a.c.page_size, kKeys);
+      constexpr int kSub = P::kSub, kPart = kKeys / kSub;  // (keys in a piece of a value tile)
+      const int box = min(a.c.page_size, is_k ? kKeys : kPart);
       uint32_t rc0 = 0, last = 0;
       bool ok = true;
       while (ok && walk.next(a, p)) {
-        const int n = p.t1 - p.t0, end = walk.w.end;
+        const int n = p.t1 - p.t0, end = walk.w.len + walk.w.n;
         const int32_t* list = a.c.table + (int64_t)walk.s * a.c.max_pages;
-        // the page that this lane copies of a tile
-        auto page_of = [&](int j) {
-          const int place = (p.t0 + j) * kKeys + lane * box;
-          return j < n && lane * box < kKeys && place < end ? list[place >> a.c.page_shift] : 0;
+        // the page that this lane copies of what begins at `place`
+        auto page_of = [&](int place, int keys) {
+          return lane * box < keys && place + lane * box < end ? list[(place + lane * box) >> a.c.page_shift] : 0;
         };
-        int id_next = page_of(0);
-        for (int j = 0; j < n; ++j) {
-          const int id = id_next;
-          id_next = page_of(j + 1);
+        const int keys = is_k ? kKeys : kPart, place0 = p.t0 * kKeys;
+        int id_next = page_of(place0, keys), id = 0;
+        for (int i = 0; ok && i < n * kSub; ++i) {
+          const int j = i / kSub, h = i % kSub;
+          const int place = place0 + (is_k ? j * kKeys : i * kPart);
+          if (!is_k || h == 0) {
+            id = id_next;
+            if (i + 1 < n * kSub) id_next = page_of(place + keys, keys);
+          }
           // (a key tile is asked for one step ahead of the value tile before it)
-          const uint32_t rc = rc0 + (MODE == kPair ? 2 * j + !is_k : is_k ? max(0, 2 * j - 1) : min(2 * j + 2, 2 * n - 1));
+          const uint32_t entry = MODE == kPair ? 2 * j + !is_k : is_k ? max(0, 2 * j - 1) : min(2 * j + 2, 2 * n - 1), rc = rc0 + entry * kSub + h;
           const int slot = rc % kRing;
           if (!hold_warp(&empty[slot], ((rc / kRing) & 1u) ^ 1u, fail)) {
             ok = false;
             break;
           }
-          const int place = (p.t0 + j) * kKeys, boxes = (min(kKeys, end - place) + box - 1) / box;
-          if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * DIM * 2));
+          const int boxes = (max(0, min(keys, end - place)) + box - 1) / box;
+          if (lane == 0) mbar_expect_tx(&full[slot], (uint32_t)(boxes * box * (is_k ? DIM / kSub : DIM) * 2));
           if (lane < boxes) {
             int row = a.no_row;
             if (id >= 0 && id < a.c.n_pages) row = id * a.page_rows + p.head * a.head_rows + (place & (a.c.page_size - 1));
             else raise_status(a.c.status, ARCS_ERR_PAGE);
             const int y = a.by_row ? row : p.head, z = a.by_row ? 0 : row;
             char* dst = ring + slot * P::kTile + lane * box * 128;
+            if (is_k) {
 #pragma unroll
-            for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kKeys * 128), map, c * 64, y, z, &full[slot]);
+              for (int c = 0; c < DIM / 64 / kSub; ++c) tile_load3(dst + c * (kKeys * 128), map, (h * (DIM / 64 / kSub) + c) * 64, y, z, &full[slot]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < DIM / 64; ++c) tile_load3(dst + c * (kPart * 128), map, c * 64, y, z, &full[slot]);
+            }
           }
           __syncwarp();
           last = rc + 1;
         }
-        rc0 += 2 * n;
+        rc0 += 2 * n * kSub;
       }
       if (!ok && lane == 0)  // the copies in flight land before the CTA's memory goes to another
         for (uint32_t i = last > (uint32_t)kRing ? last - kRing : 0; i < last; ++i) mbar_wait(&full[i % kRing], (i / kRing) & 1u);
@@ -366,95 +455,80 @@ __global__ void __maxnreg__(152)
       {
         const uint32_t on = elect_one();
         constexpr uint32_t kScores = mma_desc(128, kKeys, W::kBf16, false), kValues = mma_desc(128, DIM, W::kBf16, true);
-        Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
-        Piece p;
         uint32_t rc = 0, k = 0, turn = 0;  // (turn: a bit a score tile, the phase its barriers are in)
         bool ok = true;
-        auto scores = [&](int b, int tile, uint32_t at) {  // rows of queries `tile` x the keys in ring slot `at`
-          const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2), ka = smem_addr(ring) + at * P::kTile;
+        constexpr int kSub = P::kSub, kPart = kKeys / kSub;
+        auto commit = [&](uint64_t* bar) { mma_commit(on, bar); };
+        auto there = [&](uint32_t at) { return hold_warp(&full[at % kRing], (at / kRing) & 1u, fail); };
+        // rows of queries `tile` x the keys from ring position `at` on; `last`: the slots are free afterwards
+        auto scores = [&](int b, int tile, uint32_t at, bool last) {
+          const uint32_t qa = smem_addr(sq) + tile * (128 * DIM * 2);
 #pragma unroll
-          for (int i = 0; i < DIM / 16; ++i)
-            mma_ss(on, tmem + b * P::kScore1, smem_desc(qa + (i / 4) * 16384 + (i % 4) * 32, 16, 1024), smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores,
-                   i > 0);
+          for (int h = 0; h < kSub; ++h) {
+            const uint32_t ka = smem_addr(ring) + (at + h) % kRing * P::kTile;
+            if (kSub > 1 && !there(at + h)) return false;
+#pragma unroll
+            for (int i = 0; i < DIM / kSub / 16; ++i)
+              mma_ss(on, tmem + b * P::kScore1, smem_desc(qa + h * (DIM / kSub / 64) * 16384 + (i / 4) * 16384 + (i % 4) * 32, 16, 1024),
+                     smem_desc(ka + (i / 4) * (kKeys * 128) + (i % 4) * 32, 16, 1024), kScores, h + i > 0);
+            if (kSub > 1) commit(&empty[(at + h) % kRing]);
+          }
+          commit(&s_full[b]);
+          if (kSub == 1 && last) commit(&empty[at % kRing]);
+          return true;
         };
-        // weights of score tile b x the values in ring slot `at`: the first half of the keys as soon as their
-        // weights are there
-        auto values = [&](int b, int sums, uint32_t at, bool first) {
-          const uint32_t va = smem_addr(ring) + at * P::kTile;
+        // weights of score tile b x the values from ring position `at` on: the first half of the keys as soon
+        // as their weights are there
+        auto values = [&](int b, int sums, uint32_t at, bool first, bool last) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const uint32_t slot = (at + (kSub > 1 ? h : 0)) % kRing, va = smem_addr(ring) + slot * P::kTile + (kSub > 1 ? 0 : h * (kKeys / 32) * 2048);
+            if (kSub > 1 && !there(at + h)) return false;
             if (!hold_warp(h ? &p_full[b] : &p_half[b], (turn >> b) & 1u, fail)) return false;
             tc_fence_after();
 #pragma unroll
-            for (int i = h * kKeys / 32; i < (h + 1) * kKeys / 32; ++i)
-              mma_ts(on, tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + i * 8, smem_desc(va + i * 2048, kKeys * 128, 1024), kValues, !(first && i == 0));
+            for (int i = 0; i < kKeys / 32; ++i)
+              mma_ts(on, tmem + P::kSums + sums * DIM, tmem + b * P::kScore1 + (h * (kKeys / 32) + i) * 8, smem_desc(va + i * 2048, kPart * 128, 1024), kValues,
+                     !(first && h + i == 0));
+            if (kSub > 1 || (last && h == 1)) commit(&empty[slot]);
           }
           turn ^= 1u << b;
           return true;
         };
-        auto commit = [&](uint64_t* bar) { mma_commit(on, bar); };
         while (ok && walk.next(a, p)) {
           const int n = p.t1 - p.t0;
           const bool two = MODE == kPair && walk.w.n * a.group - p.block * kRows > 128;
-          ok = hold_warp(q_full, k & 1u, fail);
+          ok = k == 0 ? hold_warp(q_first, 0, fail) : hold_warp(q_full, (k - 1u) & 1u, fail);
           tc_fence_after();
           uint32_t k_at = 0, v_at = 0;
           for (int j = 0; ok && j <= n; ++j) {
             // (the sums of the piece before have been read: asked before the first product into them)
             if (j == 1 && k > 0 && !(ok = hold_warp(sums_free, (k - 1u) & 1u, fail))) break;
             if (MODE == kPair) {
+              // (what is copied is looked at before the weights are waited for, not between two products)
               if (j >= 1) {
-                v_at = rc % kRing;
-                ok = hold_warp(&full[v_at], (rc / kRing) & 1u, fail);
-                if (!ok) break;
-                ++rc;
+                v_at = rc++;
+                ok = there(v_at);
               }
-              if (j < n) {  // (looked at before the weights are waited for, not between the two products)
-                k_at = rc % kRing;
-                ok = hold_warp(&full[k_at], (rc / kRing) & 1u, fail);
-                if (!ok) break;
-                ++rc;
+              if (ok && j < n) {
+                k_at = rc++;
+                ok = there(k_at);
               }
-              if (j >= 1) {
-                ok = values(0, 0, v_at, j == 1);
-                if (!ok) break;
-                if (!two) commit(&empty[v_at]);
-              }
-              if (j < n) {
-                scores(0, 0, k_at);
-                commit(&s_full[0]);
-                if (!two) commit(&empty[k_at]);
-                if (!two && j == n - 1) commit(q_empty);
-              }
-              if (two && j >= 1) {
-                ok = values(1, 1, v_at, j == 1);
-                if (!ok) break;
-                commit(&empty[v_at]);
-              }
-              if (two && j < n) {
-                scores(1, 1, k_at);
-                commit(&s_full[1]);
-                commit(&empty[k_at]);
-                if (j == n - 1) commit(q_empty);
-              }
+              if (ok && j >= 1) ok = values(0, 0, v_at, j == 1, !two);
+              if (ok && j < n) ok = scores(0, 0, k_at, !two);
+              if (ok && two && j >= 1) ok = values(1, 1, v_at, j == 1, true);
+              if (ok && two && j < n) ok = scores(1, 1, k_at, true);
+              if (ok && j == n - 1) commit(q_empty);
             } else {
               if (j < n) {
-                k_at = rc % kRing;
-                ok = hold_warp(&full[k_at], (rc / kRing) & 1u, fail);
-                if (!ok) break;
-                ++rc;
-                scores(j & 1, 0, k_at);
-                commit(&s_full[j & 1]);
-                commit(&empty[k_at]);
-                if (j == n - 1) commit(q_empty);
+                ok = (kSub > 1 || there(rc)) && scores(j & 1, 0, rc, true);
+                rc += kSub;
+                if (ok && j == n - 1) commit(q_empty);
               }
-              if (j >= 1) {
+              if (ok && j >= 1) {
                 const int b = (j - 1) & 1;
-                v_at = rc % kRing;
-                ok = hold_warp(&full[v_at], (rc / kRing) & 1u, fail) && values(b, MODE == kSplit ? b : 0, v_at, MODE == kSplit ? j <= 2 : j == 1);
-                if (!ok) break;
-                ++rc;
-                commit(&empty[v_at]);
+                ok = (kSub > 1 || there(rc)) && values(b, MODE == kSplit ? b : 0, rc, MODE == kSplit ? j <= 2 : j == 1, true);
+                rc += kSub;
                 if (MODE == kShare) commit(sums_done);
               }
             }
@@ -471,29 +545,22 @@ __global__ void __maxnreg__(152)
       __syncwarp();
     } else {
       // ============================================== queries of the next piece, once the products have done with those of this one
-      Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
-      Piece p;
+      // (those of the first piece are brought by the softmax warps, which have nothing else to do then)
       uint32_t k = 0;
       while (walk.next(a, p)) {
-        if (k > 0 && !hold_warp(q_empty, (k - 1u) & 1u, fail)) break;
-        constexpr int kChunks = DIM / 8;
-        const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
-        const char* from = a.q + walk.w.off * a.q_token_stride;
-        for (int i = lane; i < rows * kChunks; i += 32) {
-          const int r = i / kChunks, c = i % kChunks, x = p.block * kRows + r, node = x / a.group, h = p.head * a.group + x - node * a.group;
-          copy16(sq + (r >> 7) * (128 * DIM * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), from + node * a.q_token_stride + h * a.q_head_stride + c * 16);
+        if (k > 0) {
+          if (!hold_warp(q_empty, (k - 1u) & 1u, fail)) break;
+          bring_queries<DIM, kRows>(a, walk.w, p, sq, lane, 32);
+          copy16_wait();
+          fence_proxy_async();
+          arrive_warp(q_full);
         }
-        copy16_wait();
-        fence_proxy_async();
-        arrive_warp(q_full);
         ++k;
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ================================================ softmax: a thread a row
-    Walk<kKeys, kRows> walk(a, u0, u1, s_first, base);
-    Piece p;
     const int grp = warp >> 2, row_t = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes of tensor memory
     const int first_row = MODE == kPair ? grp * 128 : 0, my = first_row + row_t;
@@ -503,8 +570,14 @@ __global__ void __maxnreg__(152)
     uint32_t rc0 = 0, turn = 0, k = 0, done = 0, set = 0;
     bool ok = true;
     while (ok && walk.next(a, p)) {
-      const int n = p.t1 - p.t0, len = walk.w.len, end = walk.w.end, off = walk.w.off;
+      const int n = p.t1 - p.t0, len = walk.w.len, end = len + walk.w.n, off = walk.w.off;
       const int rows = min(kRows, walk.w.n * a.group - p.block * kRows);
+      if (k == 0) {
+        bring_queries<DIM, kRows>(a, walk.w, p, sq, tid, 256);
+        copy16_wait();
+        fence_proxy_async();
+        arrive_warp(q_first);
+      }
       const bool warp_live = first_row + (warp & 3) * 32 < rows, live = my < rows;
       const int x = p.block * kRows + (live ? my : 0), node = x / a.group, head_q = p.head * a.group + x - node * a.group;
       unsigned long long bits = 0;
@@ -627,16 +700,15 @@ __global__ void __maxnreg__(152)
         if (tail && (MODE != kPair || grp == 0)) {
           // Values behind the last node are whatever the page holds, and 0 times NaN is NaN: they become
           // zeros. A node's value that is not finite, too: it is added at the end to the rows that see the node.
-          const uint32_t at = rc0 + (MODE == kPair ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1));
-          if (!hold_warp(&full[at % kRing], (at / kRing) & 1u, fail)) {
-            ok = false;
-            break;
-          }
-          char* tile = ring + (at % kRing) * P::kTile;
+          constexpr int kSub = P::kSub, kPart = kKeys / kSub;
+          const uint32_t at = rc0 + (MODE == kPair ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1)) * kSub;
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) ok = hold_warp(&full[(at + h) % kRing], ((at + h) / kRing) & 1u, fail) && ok;
+          if (!ok) break;
           const int lo = max(0, len - p0);
           for (int i = row_t; i < (kKeys - lo) * (DIM / 8); i += 128) {
             const int r = lo + i / (DIM / 8), c = i % (DIM / 8);
-            uint4* v = reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (c & 7) * 16);
+            uint4* v = reinterpret_cast<uint4*>(ring + (at + r / kPart) % kRing * P::kTile + (c >> 3) * (kPart * 128) + r % kPart * 128 + (c & 7) * 16);
             if (p0 + r >= end) {
               *v = make_uint4(0, 0, 0, 0);
               continue;
@@ -744,7 +816,7 @@ __global__ void __maxnreg__(152)
       if (tid == 0) odd[(k + 1) & 1u] = 0;
       tc_fence_before();
       arrive_warp(sums_free);
-      rc0 += 2 * n;
+      rc0 += 2 * n * P::kSub;
       done += n;
       if (MODE == kShare && warp_live && (n & 1) == grp && n > grp) ++set;  // (the piece's last tile was the other group's: nobody asked for its reference)
       ++k;
@@ -753,31 +825,6 @@ __global__ void __maxnreg__(152)
   __syncthreads();
   if (tid == 0 && *fail) raise_status(a.c.status, ARCS_ERR_TIMEOUT);
   if (warp == 9) tmem_free(tmem, 512);
-}
-
-// Where unit u lies: its slot, and the units before that. Asked by a whole warp; up to 128 slots it adds
-// them up itself (`total` too), else it searches the running sum that tree_tiles_kernel left.
-template <int KEYS, int ROWS>
-__device__ __forceinline__ uint32_t add_up(const TreeDev& a, uint32_t (&before)[4], uint32_t (&own)[4]) {
-  const int lane = threadIdx.x & 31;
-  uint32_t total = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    own[i] = 0;
-    if (i * 32 + lane < a.c.slots) own[i] = (uint32_t)slot_work<KEYS, ROWS>(a, i * 32 + lane).units;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t x = own[i];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-      if (lane >= o) x += y;
-    }
-    before[i] = total + x - own[i];
-    total += __shfl_sync(0xFFFFFFFFu, x, 31);
-  }
-  return total;
 }
 
 // The pieces of items that were cut, joined. WARPS = 4, for few items of maybe a hundred pieces each:
@@ -796,11 +843,12 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
   __shared__ float s_sum[WARPS == 4 ? 4 : 1][WARPS == 4 ? DIM : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t total = 0, base = 0, u = 0;
-  int s = WARPS == 4 ? (int)blockIdx.x / (a.c.heads * blocks) : -1;
+  int s = WARPS == 4 ? (int)blockIdx.x / (a.c.heads * blocks) : -1, extra = 0;
   const bool few = WARPS == 4 || a.c.slots <= 128;  // (few items are of few slots)
   if (few) {
+    SlotWork w[4];
     uint32_t before[4], own[4];
-    total = add_up<P::kKeys, P::kRows>(a, before, own);
+    total = add_up<P>(a, ctas, w, before, own, extra);
     u = first_unit(total, (int)blockIdx.x + 1, ctas);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -814,6 +862,7 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
   } else {
     pdl_wait();
     total = __ldcg(a.prefix + a.c.slots);
+    extra = (int)__ldcg(a.prefix + a.c.slots + 1);
     u = first_unit(total, (int)blockIdx.x + 1, ctas);
     int lo = 0, n = a.c.slots;  // the last slot with prefix <= u (those without units share theirs with the next)
     while (n > 1) {
@@ -827,22 +876,28 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     base = __ldcg(a.prefix + s);
   }
   if (s < 0 || (WARPS == 1 && u >= total)) return;
-  const SlotWork w = slot_work<P::kKeys, P::kRows>(a, s);
+  const SlotWork w = slot_work<P>(a, s);
   if (w.n == 0) return;
-  int head, block;
+  const Costs<P> costs(a, w, extra);
+  int x = (int)(u - base);
   if (WARPS == 4) {
-    const int x = (int)blockIdx.x - s * a.c.heads * blocks;
-    head = x / blocks;
-    block = x - head * blocks;
-    if (block >= w.blocks) return;
-  } else {
-    const int x = (int)(u - base) / w.tiles;
-    head = x / w.blocks;
-    block = x - head * w.blocks;
+    const int i = (int)blockIdx.x - s * a.c.heads * blocks, head = i / blocks;
+    if (i - head * blocks >= w.blocks) return;
+    x = head * costs.head + (i - head * blocks) * costs.first;
   }
-  const uint32_t begins = base + (uint32_t)((head * w.blocks + block) * w.tiles);
-  const int c0 = cta_of_unit(total, begins, ctas), c1 = cta_of_unit(total, begins + (uint32_t)w.tiles - 1u, ctas);
+  const Place at = place_of<P>(w, costs, base, x);
+  const int head = at.head, block = at.block;
+  const uint32_t tile0 = at.begins + (uint32_t)extra;  // where the item's first tile begins
+  const int c0 = cta_of_unit(total, tile0, ctas), c1 = cta_of_unit(total, tile0 + (uint32_t)((w.tiles - 1) * at.cost), ctas);
   if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return;  // not cut, or cut before
+  // (with hardly more units than CTAs some of them have no tile)
+  auto has_tile = [&](int c) {
+    if (c > c1) return false;
+    if (total >= (uint32_t)ctas * (P::kCost + 1)) return true;
+    const uint32_t u0 = first_unit(total, c, ctas), u1 = first_unit(total, c + 1, ctas);
+    const int from = max(0, (int)(u0 - tile0)), to = min((int)(u1 - tile0), w.tiles * at.cost);
+    return (from + at.cost - 1) / at.cost < (to + at.cost - 1) / at.cost;
+  };
   const int rows = min(P::kRows, w.n * a.group - block * P::kRows);
   if (few) pdl_wait();
   for (int rr = (int)blockIdx.y * (4 / WARPS) + (WARPS == 4 ? 0 : warp); rr < rows; rr += (int)gridDim.y * (4 / WARPS)) {
@@ -856,9 +911,8 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const int c = b + i;
-        // (with fewer units than CTAs some of them have none)
-        const bool there = c <= c1 && (total >= (uint32_t)ctas || first_unit(total, c, ctas) != first_unit(total, c + 1, ctas));
         const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
+        const bool there = has_tile(c);
         st[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
         for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
