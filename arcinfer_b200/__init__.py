@@ -25,5 +25,7 @@ def __getattr__(name):
         import importlib
 
         kvcache = importlib.import_module(".kvcache", __name__)
-        return kvcache if name == "kvcache" else getattr(kvcache, name)
+        value = kvcache if name == "kvcache" else getattr(kvcache, name)
+        globals()[name] = value  # (found without this function from now on: looking a name up so takes 5 us)
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

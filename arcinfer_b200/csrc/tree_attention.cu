@@ -108,7 +108,6 @@ bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const Row
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kCtas = kSmCount;
 int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair : kSplit; }
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }

@@ -54,6 +54,7 @@ static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kS
               TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
 // 8 softmax warps, two that copy keys and values, one that issues the products, one that brings the queries
 constexpr int kTileThreads = 384;
+constexpr int kCtas = kSmCount;  // one a SM
 
 struct SlotWork {
   int off, n, len, tiles, blocks;  // rows of the step, nodes, settled tokens; tiles of keys, blocks of rows a key head
@@ -890,21 +891,27 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
   const uint32_t tile0 = at.begins + (uint32_t)extra;  // where the item's first tile begins
   const int c0 = cta_of_unit(total, tile0, ctas), c1 = cta_of_unit(total, tile0 + (uint32_t)((w.tiles - 1) * at.cost), ctas);
   if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return;  // not cut, or cut before
-  // (with hardly more units than CTAs some of them have no tile)
-  auto has_tile = [&](int c) {
-    if (c > c1) return false;
-    if (total >= (uint32_t)ctas * (P::kCost + 1)) return true;
-    const uint32_t u0 = first_unit(total, c, ctas), u1 = first_unit(total, c + 1, ctas);
-    const int from = max(0, (int)(u0 - tile0)), to = min((int)(u1 - tile0), w.tiles * at.cost);
-    return (from + at.cost - 1) / at.cost < (to + at.cost - 1) / at.cost;
-  };
+  // CTA c0 + 32 i + lane has a tile of the item: bit `lane` of pieces[i] (with hardly more units than CTAs
+  // some of them have none)
+  unsigned pieces[(kCtas + 31) / 32];
+#pragma unroll
+  for (int i = 0; i < (kCtas + 31) / 32; ++i) {
+    const int c = c0 + 32 * i + lane;
+    bool has = c <= c1;
+    if (has && total < (uint32_t)ctas * (P::kCost + 1)) {
+      const uint32_t u0 = first_unit(total, c, ctas), u1 = first_unit(total, c + 1, ctas);
+      const int from = max(0, (int)(u0 - tile0)), to = min((int)(u1 - tile0), w.tiles * at.cost);
+      has = (from + at.cost - 1) / at.cost < (to + at.cost - 1) / at.cost;
+    }
+    pieces[i] = __ballot_sync(0xFFFFFFFFu, has);
+  }
   const int rows = min(P::kRows, w.n * a.group - block * P::kRows);
   if (few) pdl_wait();
   for (int rr = (int)blockIdx.y * (4 / WARPS) + (WARPS == 4 ? 0 : warp); rr < rows; rr += (int)gridDim.y * (4 / WARPS)) {
     float m = -INFINITY, l = 0.0f, o[kPer];
 #pragma unroll
     for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
-    constexpr int kAtOnce = DIM == 256 ? 2 : 4;
+    constexpr int kAtOnce = DIM == 256 ? 3 : 5;
     for (int b = c0 + (WARPS == 4 ? warp : 0) * kAtOnce; b <= c1; b += kAtOnce * WARPS) {
       float y[kAtOnce][kPer];
       float2 st[kAtOnce];
@@ -912,7 +919,11 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
       for (int i = 0; i < kAtOnce; ++i) {
         const int c = b + i;
         const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
-        const bool there = has_tile(c);
+        unsigned word = pieces[0];
+#pragma unroll
+        for (int e = 1; e < (kCtas + 31) / 32; ++e)
+          if ((c - c0) >> 5 == e) word = pieces[e];
+        const bool there = c <= c1 && ((word >> ((c - c0) & 31)) & 1u);
         st[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
         for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;

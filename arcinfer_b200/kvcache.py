@@ -4,11 +4,12 @@ that accepts a path. Tensors are torch CUDA tensors; every call enqueues on torc
 the cache's device and returns without synchronising."""
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 import torch
 
-from .capi import ArcsError, _check, _ptr, _stream, lib
+from .capi import ArcsError, _check, _stream, lib
 
 F16, BF16 = 2, 1
 TREE_MAX = 64
@@ -55,21 +56,42 @@ lib.arcs_cache_free.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
 lib.arcs_cache_compact.restype = C.c_int
 lib.arcs_cache_compact.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]
 lib.arcs_cache_append.restype = C.c_int
-lib.arcs_cache_append.argtypes = [C.POINTER(AppendArgs), C.c_void_p]
+lib.arcs_cache_append.argtypes = [C.c_void_p, C.c_void_p]
 lib.arcs_tree_attention_workspace_bytes.restype = C.c_size_t
 lib.arcs_tree_attention_workspace_bytes.argtypes = [C.c_int32] * 5
 lib.arcs_tree_attention.restype = C.c_int
-lib.arcs_tree_attention.argtypes = [C.POINTER(TreeAttentionArgs), C.c_void_p]
+lib.arcs_tree_attention.argtypes = [C.c_void_p, C.c_void_p]
 lib.arcs_accept_tree.restype = C.c_int
 lib.arcs_accept_tree.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]  # fmt: skip
 
 
+# The argument blocks of the calls of a step, packed (a ctypes structure filled field by field takes three times as
+# long, which a small batch notices); native alignment is the compiler's.
+_append_block = struct.Struct("@P3i4x3P3qPq2Pf2i4x3P")
+_attention_block = struct.Struct("@P3i4xP2qP2q3PifPN")
+assert _append_block.size == C.sizeof(AppendArgs) and _attention_block.size == C.sizeof(TreeAttentionArgs)
+_i32, _i64, _f32, _f64 = torch.int32, torch.int64, torch.float32, torch.float64
+_empty = torch.empty
+
+
 def _list(name, t, dtype, n, dev):
     """a contiguous device list of n (None: any number of) values"""
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise ArcsError(f"{name} must be a contiguous {dtype} tensor{'' if n is None else f' of {n} values'} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.device == dev and t.is_contiguous() and (n is None or t.numel() == n):
+        return t.data_ptr()
+    raise ArcsError(f"{name} must be a contiguous {dtype} tensor{'' if n is None else f' of {n} values'} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _enqueue(dev, fn, what, *args):
+    """launches on the current stream of the device, with that device current"""
+    stream = _stream(dev)
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _check(rc, what)
 
 
 class KVCache:
@@ -98,6 +120,7 @@ class KVCache:
                               _list("length", length, i32, slots, dev), _list("status", status, i32, 1, dev))
         self.ptr = C.addressof(self.args)
         self.workspace_bytes = {}
+        self.scale = 1.0 / math.sqrt(dim)
 
     @staticmethod
     def empty(layers, n_pages, heads, page_size, dim, slots, max_pages, dtype=torch.bfloat16, device="cuda"):
@@ -107,32 +130,22 @@ class KVCache:
         return KVCache(pool(), pool(), z(slots, max_pages) - 1, z(slots), z(n_pages), z(slots))
 
 
-def _call(cache, fn, what, *args):
-    """launches on the current stream of the cache's device, with that device current"""
-    dev = cache.device
-    stream = _stream(dev)
-    if dev.index is not None and dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _check(fn(*args, stream), what)
-    _check(fn(*args, stream), what)
-
-
 def cache_reserve(cache, extra):
     """arcs_cache_reserve: pages for extra[s] (int32 [slots]) more tokens behind every slot's length."""
-    _call(cache, lib.arcs_cache_reserve, "arcs_cache_reserve", cache.ptr, _list("extra", extra, torch.int32, cache.slots, cache.device))
+    _enqueue(cache.device, lib.arcs_cache_reserve, "arcs_cache_reserve", cache.ptr, _list("extra", extra, torch.int32, cache.slots, cache.device))
 
 
 def cache_fork(cache, parent):
     """arcs_cache_fork: slot s becomes a copy of slot parent[s] (int32 [slots], -1: nothing). Returns
     int32 [slots], 1 where a copy was made."""
     done = torch.empty(cache.slots, dtype=torch.int32, device=cache.device)
-    _call(cache, lib.arcs_cache_fork, "arcs_cache_fork", cache.ptr, _list("parent", parent, torch.int32, cache.slots, cache.device), done.data_ptr())
+    _enqueue(cache.device, lib.arcs_cache_fork, "arcs_cache_fork", cache.ptr, _list("parent", parent, torch.int32, cache.slots, cache.device), done.data_ptr())
     return done
 
 
 def cache_free(cache, which):
     """arcs_cache_free: every slot with which[s] != 0 (int32 [slots]) gives its pages back."""
-    _call(cache, lib.arcs_cache_free, "arcs_cache_free", cache.ptr, _list("which", which, torch.int32, cache.slots, cache.device))
+    _enqueue(cache.device, lib.arcs_cache_free, "arcs_cache_free", cache.ptr, _list("which", which, torch.int32, cache.slots, cache.device))
 
 
 def cache_compact(cache, kept, path, length_out=None):
@@ -143,16 +156,18 @@ def cache_compact(cache, kept, path, length_out=None):
     if path.dim() != 2 or path.shape[0] != cache.slots:
         raise ArcsError(f"path must be [{cache.slots}, n]")
     out = cache.length if length_out is None else length_out
-    _call(cache, lib.arcs_cache_compact, "arcs_cache_compact", cache.ptr, _list("kept", kept, torch.int32, cache.slots, dev), _list("path", path, torch.int32, None, dev),
+    _enqueue(cache.device, lib.arcs_cache_compact, "arcs_cache_compact", cache.ptr, _list("kept", kept, torch.int32, cache.slots, dev), _list("path", path, torch.int32, None, dev),
           path.shape[1], _list("length_out", out, torch.int32, cache.slots, dev))
     return out
 
 
-def _heads(name, t, T, H, cache):
+def _heads(name, t, T, H, dim, dtype, dev):
     """[T, H, dim] of the cache's type, a row's heads side by side: (address, row stride)"""
-    if t.dim() != 3 or t.shape != (T, H, cache.dim) or t.dtype != cache.dtype or t.device != cache.device or t.stride(2) != 1 or (H > 1 and t.stride(1) != cache.dim):
-        raise ArcsError(f"{name} must be {cache.dtype} [{T}, {H}, {cache.dim}] on {cache.device} with a row's heads side by side, not {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0) if T > 1 else max(t.stride(0), H * cache.dim)
+    if t.shape == (T, H, dim) and t.dtype is dtype and t.device == dev:
+        row, head, one = t.stride()
+        if one == 1 and (head == dim or H == 1):
+            return t.data_ptr(), row if T > 1 else max(row, H * dim)
+    raise ArcsError(f"{name} must be {dtype} [{T}, {H}, {dim}] on {dev} with a row's heads side by side, not {t.dtype} {tuple(t.shape)}")
 
 
 def cache_append(cache, q, k, v, node_off, pos, inv_freq, layer=0, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, q_out=None):
@@ -160,18 +175,23 @@ def cache_append(cache, q, k, v, node_off, pos, inv_freq, layer=0, q_weight=None
     [T, Hq, dim] and keys [T, heads, dim], head by head; keys and values [T, heads, dim] go to the cache.
     pos: int32 [T]; inv_freq: float64 [rot / 2]; node_off: int32 [slots + 1]. Returns the queries (q_out,
     which may be q itself, or a new tensor)."""
-    dev = cache.device
     if q.dim() != 3:
         raise ArcsError("q must be [T, Hq, dim]")
-    T, Hq = q.shape[0], q.shape[1]
+    dev, dtype, heads, dim = cache.device, cache.dtype, cache.heads, cache.dim
+    T, Hq, _ = q.shape
     if q_out is None:
-        q_out = torch.empty(T, Hq, cache.dim, dtype=cache.dtype, device=dev)
-    (qp, qs), (kp, ks), (vp, vs), (op, os_) = (_heads(n, t, T, h, cache) for n, t, h in (("q", q, Hq), ("k", k, cache.heads), ("v", v, cache.heads), ("q_out", q_out, Hq)))
-    w = [None if t is None else _list(n, t, torch.float32, cache.dim, dev) for n, t in (("q_weight", q_weight), ("k_weight", k_weight))]
-    a = AppendArgs(cache.ptr, layer, T, Hq, qp, kp, vp, qs, ks, vs, op, os_, w[0], w[1], eps, 2 * inv_freq.numel(), int(interleaved),
-                   _list("inv_freq", inv_freq, torch.float64, None, dev), _list("pos", pos, torch.int32, T, dev),
-                   _list("node_off", node_off, torch.int32, cache.slots + 1, dev))
-    _call(cache, lib.arcs_cache_append, "arcs_cache_append", C.byref(a))
+        q_out = _empty((T, Hq, dim), dtype=dtype, device=dev)
+        op, os_ = q_out.data_ptr(), Hq * dim
+    else:
+        op, os_ = _heads("q_out", q_out, T, Hq, dim, dtype, dev)
+    qp, qs = _heads("q", q, T, Hq, dim, dtype, dev)
+    kp, ks = _heads("k", k, T, heads, dim, dtype, dev)
+    vp, vs = _heads("v", v, T, heads, dim, dtype, dev)
+    block = _append_block.pack(
+        cache.ptr, layer, T, Hq, qp, kp, vp, qs, ks, vs, op, os_, 0 if q_weight is None else _list("q_weight", q_weight, _f32, dim, dev),
+        0 if k_weight is None else _list("k_weight", k_weight, _f32, dim, dev), eps, 2 * inv_freq.numel(), int(interleaved), _list("inv_freq", inv_freq, _f64, None, dev),
+        _list("pos", pos, _i32, T, dev), _list("node_off", node_off, _i32, cache.slots + 1, dev))  # fmt: skip
+    _enqueue(dev, lib.arcs_cache_append, "arcs_cache_append", block)
     return q_out
 
 
@@ -180,28 +200,37 @@ def tree_attention(q, cache, node_off, max_nodes, mask=None, layer=0, scale=None
     (bit j of a row: it sees node j of its slot) or None for chains; max_nodes: no slot has more nodes.
     scale: 1 / sqrt(dim) unless given. Returns a dict: out (like q, or the tensor given) and, with
     want_lse, lse float32 [T, Hq]."""
-    dev = cache.device
-    if q.dim() != 3 or q.shape[2] != cache.dim or q.dtype != cache.dtype or q.device != dev or q.stride(2) != 1:
-        raise ArcsError(f"q must be {cache.dtype} [T, Hq, {cache.dim}] on {dev}, a head's values side by side")
-    T, Hq = q.shape[0], q.shape[1]
+    dev, dim = cache.device, cache.dim
+    if q.dim() != 3 or q.dtype is not cache.dtype or q.device != dev:
+        raise ArcsError(f"q must be {cache.dtype} [T, Hq, {dim}] on {dev}")
+    T, Hq, d = q.shape
+    qt, qh, one = q.stride()
+    if d != dim or one != 1:
+        raise ArcsError(f"q must be [T, Hq, {dim}], a head's values side by side")
     if out is None:
-        out = torch.empty(T, Hq, cache.dim, dtype=cache.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-        raise ArcsError("out must be like q")
+        out = torch.empty_like(q) if q.is_contiguous() else _empty((T, Hq, dim), dtype=cache.dtype, device=dev)
+        ot, oh = Hq * dim, dim
+    else:
+        if out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1:
+            raise ArcsError("out must be like q")
+        ot, oh, _ = out.stride()
     r = {"out": out}
+    lse = 0
     if want_lse:
-        r["lse"] = torch.empty(T, Hq, dtype=torch.float32, device=dev)
+        r["lse"] = x = _empty((T, Hq), dtype=_f32, device=dev)
+        lse = x.data_ptr()
     nbytes = cache.workspace_bytes.get((Hq, max_nodes))
     if nbytes is None:
-        nbytes = cache.workspace_bytes[Hq, max_nodes] = lib.arcs_tree_attention_workspace_bytes(cache.slots, cache.heads, Hq, cache.dim, max_nodes)
+        nbytes = cache.workspace_bytes[Hq, max_nodes] = lib.arcs_tree_attention_workspace_bytes(cache.slots, cache.heads, Hq, dim, max_nodes)
     # (new for every call, from torch's allocator: calls on two streams, or in two graphs, never share one)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    # (a single row's or a single head's stride is of no meaning, but looked at)
-    s = [x if n > 1 else max(x, cache.dim) // 8 * 8 for t in (q, out) for x, n in ((t.stride(0), T), (t.stride(1), Hq))]
-    a = TreeAttentionArgs(cache.ptr, layer, T, Hq, q.data_ptr(), s[0], s[1], out.data_ptr(), s[2], s[3], _ptr(r.get("lse")),
-                          _list("node_off", node_off, torch.int32, cache.slots + 1, dev), None if mask is None else _list("mask", mask, torch.int64, T, dev),
-                          max_nodes, 1.0 / math.sqrt(cache.dim) if scale is None else scale, ws.data_ptr(), nbytes)
-    _call(cache, lib.arcs_tree_attention, "arcs_tree_attention", C.byref(a))
+    ws = _empty(nbytes, dtype=torch.uint8, device=dev)
+    if T < 2 or Hq < 2:  # (a single row's or a single head's stride is of no meaning, but looked at)
+        qt, ot = (x if T > 1 else max(x, dim) // 8 * 8 for x in (qt, ot))
+        qh, oh = (x if Hq > 1 else max(x, dim) // 8 * 8 for x in (qh, oh))
+    block = _attention_block.pack(
+        cache.ptr, layer, T, Hq, q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, lse, _list("node_off", node_off, _i32, cache.slots + 1, dev),
+        0 if mask is None else _list("mask", mask, _i64, T, dev), max_nodes, cache.scale if scale is None else scale, ws.data_ptr(), nbytes)  # fmt: skip
+    _enqueue(dev, lib.arcs_tree_attention, "arcs_tree_attention", block)
     return r
 
 
@@ -210,20 +239,12 @@ def accept_tree(token, draft, parent, node_off, max_nodes, status=None):
     int32 tensors: accepted, kept, next [slots], path [slots, max_nodes]. status: int32 [1], optional."""
     dev = token.device
     T, slots = token.numel(), node_off.numel() - 1
-    i32 = torch.int32
-    o = torch.empty(3 + max_nodes, slots, dtype=i32, device=dev)
-    path = o[3:].view(slots, max_nodes)
-    r = {"accepted": o[0], "kept": o[1], "next": o[2], "path": path}
-    p = o.data_ptr()
-    args = (_list("token", token, i32, None, dev), _list("draft", draft, i32, T, dev), _list("parent", parent, i32, T, dev), _list("node_off", node_off, i32, None, dev), slots, T,
-            max_nodes, p, p + 4 * slots, p + 8 * slots, p + 12 * slots, max_nodes, None if status is None else _list("status", status, i32, 1, dev))
-    stream = _stream(dev)
-    if dev.index is not None and dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _check(lib.arcs_accept_tree(*args, stream), "arcs_accept_tree")
-    else:
-        _check(lib.arcs_accept_tree(*args, stream), "arcs_accept_tree")
-    return r
+    args = (_list("token", token, _i32, None, dev), _list("draft", draft, _i32, T, dev), _list("parent", parent, _i32, T, dev), _list("node_off", node_off, _i32, None, dev))
+    accepted, kept, last = _empty((3, slots), dtype=_i32, device=dev).unbind(0)
+    path = _empty((slots, max_nodes), dtype=_i32, device=dev)
+    _enqueue(dev, lib.arcs_accept_tree, "arcs_accept_tree", *args, slots, T, max_nodes, accepted.data_ptr(), kept.data_ptr(), last.data_ptr(), path.data_ptr(), max_nodes,
+             None if status is None else _list("status", status, _i32, 1, dev))
+    return {"accepted": accepted, "kept": kept, "next": last, "path": path}
 
 
 def tree_lists(parents):
