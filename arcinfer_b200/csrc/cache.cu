@@ -165,15 +165,17 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
 }
 
 // ---------------------------------------------------------------- fork: the rest of the last page
-// A CTA takes one (layer, pool, head) of one copy: `rest` rows of dim values, 16 bytes a thread.
+// A CTA takes one (layer, pool, head) of one copy: `rest` rows of dim values, 16 bytes a thread. The
+// slots are the fast index of the grid, so that the copies of one parent read its rows at about the same
+// time, and all but the first of them find them in the L2 cache.
 __global__ void __launch_bounds__(256) fork_copy_kernel(const CacheDev c, const int32_t* __restrict__ parent, const int32_t* __restrict__ done) {
   pdl_wait();
-  const int s = blockIdx.y;
+  const int s = blockIdx.x;
   if (!done[s]) return;
   const int len = c.len[s], rest = len & (c.page_size - 1), last = len >> c.page_shift;
   if (rest == 0) return;
   const int from = c.table[(int64_t)parent[s] * c.max_pages + last], to = c.table[(int64_t)s * c.max_pages + last];
-  const int h = blockIdx.x % c.heads, lv = blockIdx.x / c.heads;
+  const int h = blockIdx.y % c.heads, lv = blockIdx.y / c.heads;
   char* pool = ((lv & 1) ? c.v : c.k) + (lv >> 1) * c.layer_stride + h * c.head_stride;
   const char* src = pool + from * c.page_stride;
   char* dst = pool + to * c.page_stride;
@@ -228,86 +230,118 @@ __global__ void __launch_bounds__(256) free_kernel(const CacheDev c, const int32
 // refuses too, and the second takes it off again.
 constexpr int32_t kRefused = 1 << 30;
 
-// Whether a slot's path can be followed; asked by a whole warp, the same answer in every lane.
+// Whether a slot's path can be followed; asked by a whole warp, the same answer in every lane. from, to:
+// where the rows of the nodes lane and lane + 32 lie and go (bytes into a (layer, pool, head)); first: the
+// first node that moves (kept: none does).
+struct Path {
+  int64_t from[2], to[2];
+  int first;
+};
 template <bool HOLDERS>
-__device__ __forceinline__ bool path_fine(const CacheDev& c, int s, int used, int kept, const int32_t* __restrict__ path, int path_stride) {
-  const int lane = threadIdx.x & 31, len = c.len[s];
+__device__ __forceinline__ bool follow(const CacheDev& c, int s, int used, int len, int kept, const int32_t* __restrict__ path, int path_stride, Path& p) {
+  const int lane = threadIdx.x & 31;
   bool fine = kept <= ARCS_TREE_MAX && kept <= path_stride && len >= 0 && used >= 0 && used <= c.max_pages && (int64_t)len <= ((int64_t)used << c.page_shift);
+  p.first = kept;
   if (fine) {
-    for (int i = lane; i < kept; i += 32) {
-      const int node = path[i], before = i ? path[i - 1] : -1;
-      if (node <= before || node >= ARCS_TREE_MAX || (int64_t)len + node >= ((int64_t)used << c.page_shift)) {
+    const int32_t* list = c.table + (int64_t)s * c.max_pages;
+    int from[2] = {0, 0}, to[2] = {0, 0}, node[2] = {-1, -1}, before[2] = {-1, -1};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = lane + 32 * e;
+      if (i < kept) {
+        node[e] = path[i];
+        if (i) before[e] = path[i - 1];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = lane + 32 * e;
+      if (i >= kept) continue;
+      // (ascending nodes have node >= i, so that the place len + i lies in the slot's pages, too; a list that
+      // is not ascending is found out by some lane, and none reads outside)
+      if (node[e] <= before[e] || node[e] < i || node[e] >= ARCS_TREE_MAX || (int64_t)len + node[e] >= ((int64_t)used << c.page_shift)) {
         fine = false;
         continue;
       }
-      const int from = c.table[(int64_t)s * c.max_pages + ((len + node) >> c.page_shift)];
-      // (the list holds ascending nodes, so node >= i and this place lies inside the slot's pages, too; the
-      // first test decides before a list that is not ascending could lead elsewhere)
-      fine = fine && from >= 0 && from < c.n_pages;
-      if (node < i) { fine = false; continue; }
-      if (node > i) {
-        const int to = c.table[(int64_t)s * c.max_pages + ((len + i) >> c.page_shift)];
-        fine = fine && to >= 0 && to < c.n_pages && (!HOLDERS || c.ref[to] == 1);
+      from[e] = list[(len + node[e]) >> c.page_shift];
+      to[e] = list[(len + i) >> c.page_shift];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = lane + 32 * e;
+      if (i >= kept || !fine) continue;
+      if (from[e] < 0 || from[e] >= c.n_pages || to[e] < 0 || to[e] >= c.n_pages) {
+        fine = false;
+        continue;
       }
+      if (node[e] > i) {
+        p.first = min(p.first, i);
+        if (HOLDERS && c.ref[to[e]] != 1) fine = false;
+      }
+      p.from[e] = from[e] * c.page_stride + ((len + node[e]) & (c.page_size - 1)) * c.token_stride;
+      p.to[e] = to[e] * c.page_stride + ((len + i) & (c.page_size - 1)) * c.token_stride;
     }
   }
+  p.first = __reduce_min_sync(0xFFFFFFFFu, p.first);
   return __all_sync(0xFFFFFFFFu, fine);
 }
 
 // Rows move towards the front only (node >= its place), and a thread keeps to one 16-byte column of
-// one (layer, pool, head): it reads up to eight rows before it writes them, in ascending order, so no
-// row is written before it has been read.
+// one (layer, pool, head) at a time: it reads up to eight rows before it writes them, in ascending order,
+// so no row is written before it has been read. The way to the rows is three dependent trips to
+// memory (path, pages, their holders), so a CTA takes as many columns as fill the machine twice
+// over rather than one a thread: 64 slots x 8192 columns took ? us with one, ? with this.
 __global__ void __launch_bounds__(256) compact_move_kernel(const CacheDev c, const int32_t* __restrict__ kept_, const int32_t* __restrict__ path_, int path_stride) {
   pdl_trigger();
   __shared__ int64_t from[ARCS_TREE_MAX], to[ARCS_TREE_MAX];
   __shared__ int s_first;
   const int s = blockIdx.y, tid = threadIdx.x;
   const int kept = kept_[s];
-  if (kept <= 0) return;
-  const int32_t* path = path_ + (int64_t)s * path_stride;
   if (tid < 32) {
-    const int used = *(volatile int32_t*)(c.used + s);
-    const bool fine = path_fine<true>(c, s, used, kept, path, path_stride);
+    const int used = *(volatile int32_t*)(c.used + s), len = c.len[s];
+    Path p;
+    const bool fine = kept <= 0 || follow<true>(c, s, used, len, kept, path_ + (int64_t)s * path_stride, path_stride, p);
     if (!fine && blockIdx.x == 0 && tid == 0 && used >= 0 && used <= c.max_pages) c.used[s] = used | kRefused;
-    int first = kept;  // nodes before it stay where they are
-    if (fine) {
-      const int len = c.len[s];
-      for (int i = tid; i < kept; i += 32) {
-        const int a = len + path[i], b = len + i;
-        if (a != b) first = min(first, i);
-        from[i] = c.table[(int64_t)s * c.max_pages + (a >> c.page_shift)] * c.page_stride + (a & (c.page_size - 1)) * c.token_stride;
-        to[i] = c.table[(int64_t)s * c.max_pages + (b >> c.page_shift)] * c.page_stride + (b & (c.page_size - 1)) * c.token_stride;
-      }
-    }
-    first = __reduce_min_sync(0xFFFFFFFFu, first);
-    if (tid == 0) s_first = first;
+    if (fine && kept > 0)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (tid + 32 * e < kept) {
+          from[tid + 32 * e] = p.from[e];
+          to[tid + 32 * e] = p.to[e];
+        }
+    if (tid == 0) s_first = fine && kept > 0 ? p.first : kept;
   }
   __syncthreads();
   const int first = s_first;
   if (first >= kept) return;
   const int row = c.dim / 8, cols = c.layers * 2 * c.heads * row;
-  const int col = blockIdx.x * 256 + tid;
-  if (col >= cols) return;
-  const int d = col % row, h = col / row % c.heads, lv = col / row / c.heads;
-  char* pool = ((lv & 1) ? c.v : c.k) + (lv >> 1) * c.layer_stride + h * c.head_stride + d * 16;
-  for (int i0 = first; i0 < kept; i0 += 8) {
-    uint4 x[8];
+  for (int col = blockIdx.x * 256 + tid; col < cols; col += gridDim.x * 256) {
+    const int d = col & (row - 1), x = col / row, h = x % c.heads, lv = x / c.heads;
+    char* pool = ((lv & 1) ? c.v : c.k) + (lv >> 1) * c.layer_stride + h * c.head_stride + d * 16;
+    for (int i0 = first; i0 < kept; i0 += 8) {
+      uint4 y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i0 + j < kept) x[j] = *reinterpret_cast<const uint4*>(pool + from[i0 + j]);
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j < kept) y[j] = *reinterpret_cast<const uint4*>(pool + from[i0 + j]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i0 + j < kept) *reinterpret_cast<uint4*>(pool + to[i0 + j]) = x[j];
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j < kept) *reinterpret_cast<uint4*>(pool + to[i0 + j]) = y[j];
+    }
   }
 }
 
+// (what it needs to know of the lists it finds out before it waits for the rows: the first launch changes
+// nothing in them but the mark)
 __global__ void __launch_bounds__(256) compact_lists_kernel(const CacheDev c, const int32_t* __restrict__ kept_, const int32_t* __restrict__ path_, int path_stride,
                                                             int32_t* len_out) {
-  pdl_wait();
   const int s = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (s >= c.slots) return;
-  const int kept = max(0, kept_[s]), len = c.len[s], used = c.used[s];
-  const bool fine = path_fine<false>(c, s, used, kept, path_ + (int64_t)s * path_stride, path_stride);
+  const int kept = max(0, kept_[s]), len = c.len[s], seen = *(volatile int32_t*)(c.used + s);
+  Path p;
+  bool fine = follow<false>(c, s, seen & ~kRefused, len, kept, path_ + (int64_t)s * path_stride, path_stride, p);
+  pdl_wait();
+  const int used = *(volatile int32_t*)(c.used + s);
+  fine = fine && used >= 0 && used <= c.max_pages;
   __syncwarp();
   if (!fine) {
     if (lane == 0) {
@@ -359,20 +393,46 @@ template <> struct Half2Of<__half> {
   }
 };
 
-// One CTA a row. The turns of the rotation are found once (in fp64: pos * inv_freq / 2 pi less its
-// whole part, so a position of any size leaves an angle exact to fp32) and shared by all heads; a
-// head is DIM / 8 neighbouring lanes with 16 bytes each.
+// One CTA a row. A head is DIM / 8 neighbouring lanes with 16 bytes each; the first four heads of a lane
+// are asked for at the start. Meanwhile one warp finds the row's place in the cache (four dependent trips
+// to memory: slot, its lists, page), and others the turns of the rotation, once for all heads: in
+// fp64, pos * inv_freq / 2 pi less its whole part, so that a position of any size leaves an angle
+// exact to fp32. What bounds it then is the memory: each value once in and once out.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
   __shared__ float2 turn[DIM / 2];
-  __shared__ int s_slot;
-  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes;
+  __shared__ int64_t s_at;  // bytes into a head of the layer; -1: nowhere, -2: not even the query
+  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes, kAhead = 4;
   const int t = blockIdx.x, tid = threadIdx.x;
+  const int lane = tid % kLanes, e0 = lane * 8, all = a.Hq + 2 * a.c.heads;
+  auto head_at = [&](int g) {
+    const char* src = g < a.Hq ? a.q + t * a.q_stride : g < a.Hq + a.c.heads ? a.k + t * a.k_stride : a.v + t * a.v_stride;
+    const int h = g < a.Hq ? g : g < a.Hq + a.c.heads ? g - a.Hq : g - a.Hq - a.c.heads;
+    return reinterpret_cast<const uint4*>(src + (int64_t)h * (DIM * 2) + lane * 16);
+  };
+  uint4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int g = tid / kLanes + i * kGroups;
+    ahead[i] = make_uint4(0, 0, 0, 0);
+    if (g < all) ahead[i] = *head_at(g);
+  }
   if (tid < 32) {
     const int s = slot_of_row(a.node_off, a.c.slots, t);
-    if (tid == 0) s_slot = s;
-  }
-  if (tid >= 128 && tid - 128 < a.rot / 2) {
+    int64_t at = -2;
+    if (s >= 0 && tid == 0) {
+      const int64_t place = (int64_t)a.c.len[s] + (t - a.node_off[s]), list = place >> a.c.page_shift;
+      int page = -1;
+      if (place >= 0 && list < a.c.used[s] && list < a.c.max_pages) page = a.c.table[(int64_t)s * a.c.max_pages + list];
+      if (page < 0 || page >= a.c.n_pages) {
+        at = -1;
+        raise_status(a.c.status, ARCS_ERR_PAGE);
+      } else {
+        at = page * a.c.page_stride + (place & (a.c.page_size - 1)) * a.c.token_stride;
+      }
+    }
+    if (tid == 0) s_at = at;
+  } else if (tid >= 128 && tid - 128 < a.rot / 2) {
     const int i = tid - 128;
     const double turns = (double)a.pos[t] * a.inv_freq[i] * 0.15915494309189533577;
     float sn, cs;
@@ -380,72 +440,75 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
     turn[i] = make_float2(cs, sn);
   }
   __syncthreads();
-  const int s = s_slot;
-  if (s < 0) return;  // behind the last slot's rows
-  const int64_t place = (int64_t)a.c.len[s] + (t - a.node_off[s]), list = place >> a.c.page_shift;
-  int page = -1;
-  if (place >= 0 && list < a.c.used[s] && list < a.c.max_pages) page = a.c.table[(int64_t)s * a.c.max_pages + list];
-  if (page < 0 || page >= a.c.n_pages) {
-    page = -1;
-    if (tid == 0) raise_status(a.c.status, ARCS_ERR_PAGE);
-  }
-  const int64_t at = page * a.c.page_stride + (place & (a.c.page_size - 1)) * a.c.token_stride;
-  const int lane = tid % kLanes, e0 = lane * 8;
-  const int all = a.Hq + 2 * a.c.heads;
-  for (int g0 = 0; g0 < all; g0 += kGroups) {
-    const int g = g0 + tid / kLanes;
-    const bool live = g < all;
-    const bool is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
-    const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
-    const char* src = is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (live) x = *reinterpret_cast<const uint4*>(src + (int64_t)h * (DIM * 2) + lane * 16);
-    float y[8];
+  const int64_t at = s_at;
+  if (at == -2) return;  // behind the last slot's rows
+  const int half = a.rot / 2;
+  for (int g0 = 0; g0 < all; g0 += kGroups * kAhead) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = Half2Of<T>::widen(j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w);
-      y[2 * j] = f.x;
-      y[2 * j + 1] = f.y;
-    }
-    float ss = 0.0f;
+    for (int i = 0; i < kAhead; ++i) {
+      const int g = g0 + i * kGroups + tid / kLanes;
+      if (g0 + i * kGroups >= all) break;
+      const bool live = g < all, is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
+      uint4 x = ahead[i];
+      if (g + kGroups * kAhead < all) ahead[i] = *head_at(g + kGroups * kAhead);
+      const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
+      if (!__all_sync(0xFFFFFFFFu, is_v || !live)) {
+        float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
-    if (w && live) {
-      const float r = 1.0f / sqrtf(ss * (1.0f / DIM) + a.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * r * __ldg(w + e0 + j);
-    }
-    const int half = a.rot / 2;
-    if (a.interleaved) {
-      if (!is_v && e0 < a.rot) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float2 f = turn[(e0 + j) / 2];
-          const float u = y[j] * f.x - y[j + 1] * f.y;
-          y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
-          y[j] = u;
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = Half2Of<T>::widen(j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w);
+          y[2 * j] = f.x;
+          y[2 * j + 1] = f.y;
         }
-      }
-    } else if (a.rot) {
-      // the pair's other value is in the lane rot / 16 further, or before
-      const bool first = e0 < half;
-      const int other = first ? lane + half / 8 : e0 < a.rot ? lane - half / 8 : lane;
+        const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+        if (a.q_weight || a.k_weight) {
+          float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
-        if (!is_v && e0 < a.rot) {
-          const float2 f = turn[(first ? e0 : e0 - half) + j];
-          y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
+          for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+          if (w && live) {
+            const float r = rsqrtf(ss * (1.0f / DIM) + a.eps);
+            const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + e0)), w1 = __ldg(reinterpret_cast<const float4*>(w + e0) + 1);
+            y[0] *= r * w0.x;
+            y[1] *= r * w0.y;
+            y[2] *= r * w0.z;
+            y[3] *= r * w0.w;
+            y[4] *= r * w1.x;
+            y[5] *= r * w1.y;
+            y[6] *= r * w1.z;
+            y[7] *= r * w1.w;
+          }
         }
+        if (a.interleaved) {
+          if (e0 < a.rot) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+              const float2 f = turn[(e0 + j) / 2];
+              const float u = y[j] * f.x - y[j + 1] * f.y;
+              y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
+              y[j] = u;
+            }
+          }
+        } else if (a.rot) {
+          // the pair's other value is in the lane rot / 16 further, or before
+          const bool first = e0 < half;
+          const int other = first ? lane + half / 8 : e0 < a.rot ? lane - half / 8 : lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
+            if (e0 < a.rot) {
+              const float2 f = turn[(first ? e0 : e0 - half) + j];
+              y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
+            }
+          }
+        }
+        if (!is_v) x = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
       }
+      if (!live || (!is_q && at < 0)) continue;
+      char* dst = is_q ? a.q_out + t * a.q_out_stride + (int64_t)h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
+      *reinterpret_cast<uint4*>(dst + lane * 16) = x;
     }
-    if (!live || (!is_q && page < 0)) continue;
-    if (!is_v) x = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
-    char* dst = is_q ? a.q_out + t * a.q_out_stride + (int64_t)h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
-    *reinterpret_cast<uint4*>(dst + lane * 16) = x;
   }
 }
 
@@ -469,7 +532,8 @@ extern "C" int arcs_cache_fork(const arcs_cache* cache, const int32_t* parent, i
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   alloc_kernel<true><<<1, kAllocThreads, 0, st>>>(c, parent, done);
   if (int rc = check_launch("cache_fork")) return rc;
-  const dim3 grid((unsigned)(c.layers * 2 * c.heads), (unsigned)c.slots);
+  if ((int64_t)c.layers * 2 * c.heads > 65535) return bad_argument("cache_fork", "layers x heads is above 32767");
+  const dim3 grid((unsigned)c.slots, (unsigned)(c.layers * 2 * c.heads));
   launch_behind(fork_copy_kernel, grid, dim3(256), 0, st, c, parent, done);
   return check_launch("cache_fork");
 }
@@ -490,7 +554,8 @@ extern "C" int arcs_cache_compact(const arcs_cache* cache, const int32_t* kept, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t cols = (int64_t)c.layers * 2 * c.heads * (c.dim / 8);
   if (cols > 0x7FFFFF00ll) return bad_argument("cache_compact", "layers x heads x dim is too large");
-  compact_move_kernel<<<dim3((unsigned)((cols + 255) / 256), (unsigned)c.slots), 256, 0, st>>>(c, kept, path, path_stride);
+  const int64_t most = (cols + 255) / 256, fill = (4 * kSmCount + c.slots - 1) / c.slots;
+  compact_move_kernel<<<dim3((unsigned)(most < fill ? most : fill), (unsigned)c.slots), 256, 0, st>>>(c, kept, path, path_stride);
   if (int rc = check_launch("cache_compact")) return rc;
   launch_behind(compact_lists_kernel, dim3((unsigned)((c.slots + 7) / 8)), dim3(256), 0, st, c, kept, path, path_stride, len_out);
   return check_launch("cache_compact");
@@ -509,7 +574,8 @@ extern "C" int arcs_cache_append(const arcs_append_args* g, void* stream) {
   const int64_t qrow = (int64_t)g->Hq * c->dim, krow = (int64_t)c->heads * c->dim;
   if (((g->q_stride | g->k_stride | g->v_stride | g->q_out_stride) & 7) || g->q_stride < qrow || g->q_out_stride < qrow || g->k_stride < krow || g->v_stride < krow)
     return bad_argument("cache_append", "a stride is not a multiple of 8 elements, or shorter than a row");
-  if ((reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->k) | reinterpret_cast<uintptr_t>(g->v) | reinterpret_cast<uintptr_t>(g->q_out)) & 15)
+  if ((reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->k) | reinterpret_cast<uintptr_t>(g->v) | reinterpret_cast<uintptr_t>(g->q_out) |
+       reinterpret_cast<uintptr_t>(g->q_weight) | reinterpret_cast<uintptr_t>(g->k_weight)) & 15)
     return bad_argument("cache_append", "a tensor is not 16-byte aligned");
   if (!(g->eps >= 0.0f)) return bad_argument("cache_append", "eps is negative");
   AppendDev a;

@@ -462,8 +462,8 @@ typedef struct {
   int64_t q_stride, k_stride, v_stride;   /* multiples of 8; the tensors 16-byte aligned */
   void* q_out;                 /* [T][Hq][dim], rows q_out_stride apart; may be q itself */
   int64_t q_out_stride;
-  const float* q_weight;       /* [dim], or NULL: queries are not normalised */
-  const float* k_weight;       /* [dim], or NULL: keys are not normalised */
+  const float* q_weight;       /* [dim], 16-byte aligned, or NULL: queries are not normalised */
+  const float* k_weight;       /* [dim], 16-byte aligned, or NULL: keys are not normalised */
   float eps;
   int32_t rot;                 /* values rotated: 0 .. dim, a multiple of 16 */
   int32_t interleaved;

@@ -62,7 +62,7 @@ def test_lists():
 
 @pytest.mark.parametrize("bad", [dict(layer=-1), dict(layer=2), dict(T=-1), dict(Hq=0), dict(q=None), dict(k=None), dict(v=None), dict(q_out=None), dict(pos=None), dict(node_off=None),
                                  dict(inv_freq=None), dict(rot=8), dict(rot=80), dict(rot=-16), dict(q_stride=252), dict(q_stride=128), dict(k_stride=64), dict(v_stride=64),
-                                 dict(q_out_stride=128), dict(q=P + 8), dict(k=P + 4), dict(v=P + 2), dict(q_out=P + 8), dict(eps=-1.0), dict(eps=float("nan"))], ids=str)  # fmt: skip
+                                 dict(q_out_stride=128), dict(q=P + 8), dict(k=P + 4), dict(v=P + 2), dict(q_out=P + 8), dict(q_weight=P + 4), dict(k_weight=P + 8), dict(eps=-1.0), dict(eps=float("nan"))], ids=str)  # fmt: skip
 def test_append(bad):
     c = _cache()
     assert ab.lib.arcs_cache_append(C.byref(_append(c, **bad)), None) == 1
