@@ -47,52 +47,62 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (FORK) pdl_trigger();
 
+  // (the first stretch of the pages' counts is on its way before anything else is known)
+  const int w0 = warp * 256;
+  int32_t count[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) count[j] = w0 + j * 32 + lane < c.n_pages ? c.ref[w0 + j * 32 + lane] : 1;
+
+  // what each slot needs: pre[s], and base[s]
+  for (int s = tid; s < c.slots; s += kAllocThreads) {
+    const int a = ask[s], used = c.used[s], len = c.len[s];
+    int need = 0, at = -1;
+    if (!FORK && a > 0) {
+      if (used < 0 || used > c.max_pages || len < 0) {
+        raise_status(c.status, ARCS_ERR_PAGE);
+      } else {
+        const int64_t want = ((int64_t)len + a + c.page_size - 1) >> c.page_shift;
+        if (want > c.max_pages) raise_status(c.status, ARCS_ERR_FULL);
+        else if (want > used) { need = (int)want - used; at = used; }
+      }
+    }
+    if (FORK && a >= 0) {
+      bool fine = a < c.slots && a != s && used == 0;
+      if (fine) {
+        const int from_len = c.len[a], from_used = c.used[a];
+        fine = ask[a] < 0 && from_len >= 0 && from_used >= 0 && from_used <= c.max_pages && (int64_t)from_len <= ((int64_t)from_used << c.page_shift);
+        if (fine) { at = from_len >> c.page_shift; need = (from_len & (c.page_size - 1)) != 0; }
+      }
+      if (!fine) raise_status(c.status, ARCS_ERR_PAGE);
+    }
+    pre[s] = need;
+    base[s] = at;
+  }
+  __syncthreads();
+  if (FORK) {  // the lists of pages are looked over by a warp each, before anything is promised
+    for (int s = warp; s < c.slots; s += kAllocThreads / 32) {
+      const int at = base[s], n = at + pre[s];
+      if (at < 0) continue;
+      const int32_t* from = c.table + (int64_t)ask[s] * c.max_pages;
+      bool fine = true;
+      for (int i = lane; i < n; i += 32) {
+        const int p = from[i];
+        fine = fine && p >= 0 && p < c.n_pages && c.ref[p] > 0;
+      }
+      if (!__all_sync(0xFFFFFFFFu, fine) && lane == 0) {
+        base[s] = -1;
+        pre[s] = 0;
+        raise_status(c.status, ARCS_ERR_PAGE);
+      }
+    }
+    __syncthreads();
+  }
   int sum = 0;
   for (int s0 = 0; s0 < c.slots; s0 += kAllocThreads) {
     const int s = s0 + tid;
-    int need = 0, at = -1;
-    if (s < c.slots) {
-      const int a = ask[s];
-      if (!FORK && a > 0) {
-        const int used = c.used[s], len = c.len[s];
-        if (used < 0 || used > c.max_pages || len < 0) {
-          raise_status(c.status, ARCS_ERR_PAGE);
-        } else {
-          const int64_t want = ((int64_t)len + a + c.page_size - 1) >> c.page_shift;
-          if (want > c.max_pages) raise_status(c.status, ARCS_ERR_FULL);
-          else if (want > used) { need = (int)want - used; at = used; }
-        }
-      }
-      if (FORK && a >= 0) {
-        bool fine = a < c.slots && a != s && c.used[s] == 0;
-        if (fine) {
-          const int len = c.len[a], used = c.used[a];
-          fine = ask[a] < 0 && len >= 0 && used >= 0 && used <= c.max_pages && (int64_t)len <= ((int64_t)used << c.page_shift);
-          if (fine) { at = len >> c.page_shift; need = (len & (c.page_size - 1)) != 0; }
-        }
-        if (!fine) raise_status(c.status, ARCS_ERR_PAGE);
-      }
-    }
-    if (FORK) {  // (the lists of pages are looked over by a warp each, before anything is promised)
-      for (int q = 0; q < 32; ++q) {
-        const int sq = s0 + warp * 32 + q, atq = __shfl_sync(0xFFFFFFFFu, at, q), needq = __shfl_sync(0xFFFFFFFFu, need, q);
-        if (atq < 0) continue;
-        const int32_t* from = c.table + (int64_t)ask[sq] * c.max_pages;
-        bool fine = true;
-        for (int i = lane; i < atq + needq; i += 32) {
-          const int p = from[i];
-          fine = fine && p >= 0 && p < c.n_pages && c.ref[p] > 0;
-        }
-        if (!__all_sync(0xFFFFFFFFu, fine) && lane == q) {
-          at = -1;
-          need = 0;
-          raise_status(c.status, ARCS_ERR_PAGE);
-        }
-      }
-    }
     int all;
-    const int before = block_scan_exclusive(need, warp_sums, &all);
-    if (s < c.slots) { pre[s] = sum + before; base[s] = at; }
+    const int before = block_scan_exclusive(s < c.slots ? pre[s] : 0, warp_sums, &all);
+    if (s < c.slots) pre[s] = sum + before;
     sum += all;
   }
   if (tid == 0) pre[c.slots] = sum;
@@ -102,11 +112,14 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
   for (int p0 = 0; p0 < c.n_pages && found < sum; p0 += kAllocThreads * 8) {
     unsigned b[8];
     int mine = 0;
-    const int w0 = p0 + warp * 256;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int p = w0 + j * 32 + lane;
-      b[j] = __ballot_sync(0xFFFFFFFFu, p < c.n_pages && c.ref[p] == 0);
+      const int p = p0 + w0 + j * 32 + lane;
+      if (p0 > 0) count[j] = p < c.n_pages ? c.ref[p] : 1;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      b[j] = __ballot_sync(0xFFFFFFFFu, count[j] == 0);
       mine += __popc(b[j]);
     }
     int all;
@@ -124,7 +137,7 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
         if (pre[mid] <= r) lo = mid;
         else hi = mid;
       }
-      const int p = w0 + j * 32 + lane;
+      const int p = p0 + w0 + j * 32 + lane;
       c.table[(int64_t)lo * c.max_pages + base[lo] + r - pre[lo]] = p;
       c.ref[p] = 1;
     }
@@ -393,65 +406,81 @@ template <> struct Half2Of<__half> {
   }
 };
 
-// One CTA a row. A head is DIM / 8 neighbouring lanes with 16 bytes each; the first four heads of a lane
-// are asked for at the start. Meanwhile one warp finds the row's place in the cache (four dependent trips
-// to memory: slot, its lists, page), and others the turns of the rotation, once for all heads: in
-// fp64, pos * inv_freq / 2 pi less its whole part, so that a position of any size leaves an angle
-// exact to fp32. What bounds it then is the memory: each value once in and once out.
+// A CTA takes `per` rows (up to four: with many rows the way to a row's place, four dependent trips to memory,
+// is what bounds a CTA with one). Four warps find the places, the others the turns of the rotation, once
+// for all heads: in fp64, pos * inv_freq / 2 pi less its whole part, so that a position of any size
+// leaves an angle exact to fp32. Meanwhile the first heads are on their way: a head is DIM / 8 neighbouring
+// lanes with 16 bytes each, and a lane's next kAhead heads are always asked for. What bounds it then is
+// the memory: each value once in and once out.
+constexpr int kAppendRows = 4;
 template <typename T, int DIM>
-__global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
-  __shared__ float2 turn[DIM / 2];
-  __shared__ int64_t s_at;  // bytes into a head of the layer; -1: nowhere, -2: not even the query
-  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes, kAhead = 4;
-  const int t = blockIdx.x, tid = threadIdx.x;
-  const int lane = tid % kLanes, e0 = lane * 8, all = a.Hq + 2 * a.c.heads;
-  auto head_at = [&](int g) {
-    const char* src = g < a.Hq ? a.q + t * a.q_stride : g < a.Hq + a.c.heads ? a.k + t * a.k_stride : a.v + t * a.v_stride;
-    const int h = g < a.Hq ? g : g < a.Hq + a.c.heads ? g - a.Hq : g - a.Hq - a.c.heads;
-    return reinterpret_cast<const uint4*>(src + (int64_t)h * (DIM * 2) + lane * 16);
+__global__ void __launch_bounds__(256, 5) append_kernel(const AppendDev a, int per) {
+  __shared__ float2 turn[kAppendRows][DIM / 2];
+  __shared__ int64_t s_at[kAppendRows];  // bytes into a head of the layer; -1: nowhere, -2: not even the query
+  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes, kAhead = 3;
+  const int t0 = blockIdx.x * per, rows = min(per, a.T - t0), tid = threadIdx.x;
+  const int lane = tid % kLanes, e0 = lane * 8, all = a.Hq + 2 * a.c.heads, half = a.rot / 2;
+  struct At {  // a row of this CTA's and a head of it
+    int r, g;
+  };
+  auto forward = [&](At& p) {
+    for (p.g += kGroups; p.g >= all; p.g -= all) ++p.r;
+  };
+  auto load = [&](const At& p) {
+    const int64_t t = t0 + p.r;
+    const char* src = p.g < a.Hq ? a.q + t * a.q_stride : p.g < a.Hq + a.c.heads ? a.k + t * a.k_stride : a.v + t * a.v_stride;
+    const int h = p.g < a.Hq ? p.g : p.g < a.Hq + a.c.heads ? p.g - a.Hq : p.g - a.Hq - a.c.heads;
+    return *reinterpret_cast<const uint4*>(src + h * (DIM * 2) + lane * 16);
   };
   uint4 ahead[kAhead];
+  At now{0, tid / kLanes - kGroups}, next;
+  forward(now);
+  next = now;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const int g = tid / kLanes + i * kGroups;
     ahead[i] = make_uint4(0, 0, 0, 0);
-    if (g < all) ahead[i] = *head_at(g);
+    if (next.r < rows) ahead[i] = load(next);
+    forward(next);
   }
-  if (tid < 32) {
-    const int s = slot_of_row(a.node_off, a.c.slots, t);
-    int64_t at = -2;
-    if (s >= 0 && tid == 0) {
-      const int64_t place = (int64_t)a.c.len[s] + (t - a.node_off[s]), list = place >> a.c.page_shift;
-      int page = -1;
-      if (place >= 0 && list < a.c.used[s] && list < a.c.max_pages) page = a.c.table[(int64_t)s * a.c.max_pages + list];
-      if (page < 0 || page >= a.c.n_pages) {
-        at = -1;
-        raise_status(a.c.status, ARCS_ERR_PAGE);
-      } else {
-        at = page * a.c.page_stride + (place & (a.c.page_size - 1)) * a.c.token_stride;
+  if (tid < 32 * kAppendRows) {
+    const int r = tid / 32;
+    if (r < rows) {
+      const int t = t0 + r, s = slot_of_row(a.node_off, a.c.slots, t);
+      if (tid % 32 == 0) {
+        int64_t at = -2;
+        if (s >= 0) {
+          const int64_t place = (int64_t)a.c.len[s] + (t - a.node_off[s]), list = place >> a.c.page_shift;
+          int page = -1;
+          if (place >= 0 && list < a.c.used[s] && list < a.c.max_pages) page = a.c.table[(int64_t)s * a.c.max_pages + list];
+          if (page < 0 || page >= a.c.n_pages) {
+            at = -1;
+            raise_status(a.c.status, ARCS_ERR_PAGE);
+          } else {
+            at = page * a.c.page_stride + (place & (a.c.page_size - 1)) * a.c.token_stride;
+          }
+        }
+        s_at[r] = at;
       }
     }
-    if (tid == 0) s_at = at;
-  } else if (tid >= 128 && tid - 128 < a.rot / 2) {
-    const int i = tid - 128;
-    const double turns = (double)a.pos[t] * a.inv_freq[i] * 0.15915494309189533577;
-    float sn, cs;
-    sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
-    turn[i] = make_float2(cs, sn);
+  } else if (half > 0) {
+    for (int i = tid - 32 * kAppendRows; i < rows * half; i += 256 - 32 * kAppendRows) {
+      const int r = i / half, e = i - r * half;
+      const double turns = (double)a.pos[t0 + r] * a.inv_freq[e] * 0.15915494309189533577;
+      float sn, cs;
+      sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
+      turn[r][e] = make_float2(cs, sn);
+    }
   }
   __syncthreads();
-  const int64_t at = s_at;
-  if (at == -2) return;  // behind the last slot's rows
-  const int half = a.rot / 2;
-  for (int g0 = 0; g0 < all; g0 += kGroups * kAhead) {
+  // (the lanes of a warp may be at different heads, but all go on until the last of them has none)
+  while (__any_sync(0xFFFFFFFFu, now.r < rows)) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int g = g0 + i * kGroups + tid / kLanes;
-      if (g0 + i * kGroups >= all) break;
-      const bool live = g < all, is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
+      const bool live = now.r < rows, is_q = now.g < a.Hq, is_v = now.g >= a.Hq + a.c.heads;
+      const int h = is_q ? now.g : is_v ? now.g - a.Hq - a.c.heads : now.g - a.Hq;
       uint4 x = ahead[i];
-      if (g + kGroups * kAhead < all) ahead[i] = *head_at(g + kGroups * kAhead);
-      const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
+      if (next.r < rows) ahead[i] = load(next);
+      forward(next);
       if (!__all_sync(0xFFFFFFFFu, is_v || !live)) {
         float y[8];
 #pragma unroll
@@ -480,11 +509,12 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
             y[7] *= r * w1.w;
           }
         }
+        const float2* turns = turn[live ? now.r : 0];
         if (a.interleaved) {
           if (e0 < a.rot) {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-              const float2 f = turn[(e0 + j) / 2];
+              const float2 f = turns[(e0 + j) / 2];
               const float u = y[j] * f.x - y[j + 1] * f.y;
               y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
               y[j] = u;
@@ -498,16 +528,21 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendDev a) {
           for (int j = 0; j < 8; ++j) {
             const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
             if (e0 < a.rot) {
-              const float2 f = turn[(first ? e0 : e0 - half) + j];
+              const float2 f = turns[(first ? e0 : e0 - half) + j];
               y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
             }
           }
         }
         if (!is_v) x = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
       }
-      if (!live || (!is_q && at < 0)) continue;
-      char* dst = is_q ? a.q_out + t * a.q_out_stride + (int64_t)h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
-      *reinterpret_cast<uint4*>(dst + lane * 16) = x;
+      if (live) {
+        const int64_t at = s_at[now.r];
+        if (at >= (is_q ? -1 : 0)) {
+          char* dst = is_q ? a.q_out + (t0 + now.r) * a.q_out_stride + h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
+          *reinterpret_cast<uint4*>(dst + lane * 16) = x;
+        }
+      }
+      forward(now);
     }
   }
 }
@@ -601,12 +636,15 @@ extern "C" int arcs_cache_append(const arcs_append_args* g, void* stream) {
   a.pos = g->pos;
   a.node_off = g->node_off;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)g->T;
+  // (rows enough to give every SM its five CTAs of four rows: then four. 500 rows took ? us with one, ? with four;
+  // 14,700 rows ? and ? us)
+  const int per = g->T >= kSmCount * 5 * kAppendRows ? kAppendRows : 1;
+  const unsigned grid = (unsigned)((g->T + per - 1) / per);
 #define ARCS_LAUNCH(TYPE)                                                     \
   do {                                                                        \
-    if (c->dim == 64) append_kernel<TYPE, 64><<<grid, 256, 0, st>>>(a);       \
-    else if (c->dim == 128) append_kernel<TYPE, 128><<<grid, 256, 0, st>>>(a); \
-    else append_kernel<TYPE, 256><<<grid, 256, 0, st>>>(a);                   \
+    if (c->dim == 64) append_kernel<TYPE, 64><<<grid, 256, 0, st>>>(a, per);       \
+    else if (c->dim == 128) append_kernel<TYPE, 128><<<grid, 256, 0, st>>>(a, per); \
+    else append_kernel<TYPE, 256><<<grid, 256, 0, st>>>(a, per);                   \
   } while (0)
   if (c->dtype == ARCS_BF16) ARCS_LAUNCH(__nv_bfloat16);
   else ARCS_LAUNCH(__half);

@@ -876,21 +876,23 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     s = lo;
     base = __ldcg(a.prefix + s);
   }
-  if (s < 0 || (WARPS == 1 && u >= total)) return;
+  // (every CTA waits before it ends: what follows on the stream begins when this grid is done, and must not
+  // find the tiles still at work)
+  if (s < 0 || (WARPS == 1 && u >= total)) return pdl_wait();
   const SlotWork w = slot_work<P>(a, s);
-  if (w.n == 0) return;
+  if (w.n == 0) return pdl_wait();
   const Costs<P> costs(a, w, extra);
   int x = (int)(u - base);
   if (WARPS == 4) {
     const int i = (int)blockIdx.x - s * a.c.heads * blocks, head = i / blocks;
-    if (i - head * blocks >= w.blocks) return;
+    if (i - head * blocks >= w.blocks) return pdl_wait();
     x = head * costs.head + (i - head * blocks) * costs.first;
   }
   const Place at = place_of<P>(w, costs, base, x);
   const int head = at.head, block = at.block;
   const uint32_t tile0 = at.begins + (uint32_t)extra;  // where the item's first tile begins
   const int c0 = cta_of_unit(total, tile0, ctas), c1 = cta_of_unit(total, tile0 + (uint32_t)((w.tiles - 1) * at.cost), ctas);
-  if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return;  // not cut, or cut before
+  if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return pdl_wait();  // not cut, or cut before
   // CTA c0 + 32 i + lane has a tile of the item: bit `lane` of pieces[i] (with hardly more units than CTAs
   // some of them have none)
   unsigned pieces[(kCtas + 31) / 32];
