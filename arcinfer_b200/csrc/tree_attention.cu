@@ -123,7 +123,7 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a,
   const int blocks = (a.max_nodes * a.group + P::kRows - 1) / P::kRows;
   const int64_t items = (int64_t)a.c.slots * a.c.heads * blocks;
   if (items <= kCtas / 2) launch_behind(join_kernel<T, DIM, MODE, 4>, dim3((unsigned)items, (unsigned)a.part_rows), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
-  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3(kCtas - 1, (unsigned)(a.part_rows + 15) / 16), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
+  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3(kCtas - 1, (unsigned)(a.part_rows + 7) / 8), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
   return check_launch("tree_attention");
 }
 
@@ -193,7 +193,7 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
     const size_t blocks = (size_t)kCtas * 2 * a.part_rows;
     a.prefix = reinterpret_cast<uint32_t*>(ws);
     a.part_stat = reinterpret_cast<float2*>(ws + round16(((size_t)c->slots + 2) * 4));
-    a.part = reinterpret_cast<float*>(ws + round16(((size_t)c->slots + 2) * 4) + round16(blocks * 8));
+    a.part = reinterpret_cast<float4*>(ws + round16(((size_t)c->slots + 2) * 4) + round16(blocks * 8));
 #define ARCS_LAUNCH(TYPE)                                                                \
   do {                                                                                   \
     if (c->dim == 256) return launch_tiles<TYPE, 256, kShare>(mk, mv, a, st);           \

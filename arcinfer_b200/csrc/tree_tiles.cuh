@@ -21,7 +21,7 @@ struct TreeDev {
   int32_t part_rows;                             // rows of a block of partial results
   uint32_t* prefix;                              // [slots + 1] units of work before a slot
   float2* part_stat;                             // [CTAs][2][part_rows] (maximum in log2, sum)
-  float* part;                                   // [CTAs][2][part_rows][dim]
+  float4* part;                                  // [CTAs][2][dim / 4][part_rows]: a warp's rows side by side where they are written
 };
 
 // How the two groups of softmax warps share the work. kSplit: one tile of rows, the tiles of keys
@@ -46,9 +46,10 @@ struct TilePlan {
   static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 1024;
   static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
   static constexpr uint32_t kSums = 256;
-  // What a tile of keys costs: 3 for two tiles of rows, 2 where an item has only one of its two; and an
-  // item for its beginning and end, about as much as two tiles.
-  static constexpr int kCost = MODE == kPair ? 3 : 1, kCostOne = MODE == kPair ? 2 : 1, kItemCost = 2 * kCost;
+  // What a tile of keys costs, and an item for its beginning and end (queries, the last tile's way through,
+  // results): fitted to the ends of all CTAs. With two tiles of rows 2.73 us, with one of them 2.28, an item
+  // 8.8; with one tile of rows 1.35 us and an item 5.0.
+  static constexpr int kCost = MODE == kPair ? 6 : 1, kCostOne = MODE == kPair ? 5 : 1, kItemCost = MODE == kPair ? 18 : 4;
 };
 static_assert(TilePlan<128, kSplit>::kSmem <= 232448 && TilePlan<128, kPair>::kSmem <= 232448 && TilePlan<256, kShare>::kSmem <= 232448 &&
               TilePlan<64, kPair>::kSmem <= 232448, "227 KB of shared memory");
@@ -213,6 +214,28 @@ template <> struct Weight<__half> {
     return __half2float(h);
   }
 };
+
+// Among four neighbouring lanes: lane b gets part b of all four lanes' y (y[e]: that of lane e).
+__device__ __forceinline__ void swap_words(uint32_t& low, uint32_t& high, bool up, int mask) {
+  // the lane with the bit gives the lower of two, the other the upper
+  const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? low : high, mask);
+  low = up ? got : low;
+  high = up ? high : got;
+}
+__device__ __forceinline__ void transpose4(uint4 (&y)[4], int lane) {
+#pragma unroll
+  for (int s = 1; s < 4; s <<= 1) {
+    const bool up = (lane & s) != 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e & s) continue;
+      swap_words(y[e].x, y[e | s].x, up, s);
+      swap_words(y[e].y, y[e | s].y, up, s);
+      swap_words(y[e].z, y[e | s].z, up, s);
+      swap_words(y[e].w, y[e | s].w, up, s);
+    }
+  }
+}
 
 // weight * sum, where the weight may have been rounded to nothing and the sum may be infinite
 __device__ __forceinline__ float weighed(float w, float o) { return w == 0.0f ? (fabsf(o) <= 3.402823466e38f ? 0.0f : o) : w * o; }
@@ -638,11 +661,11 @@ __global__ void __maxnreg__(152)
             handed[row_t] = now;
             arrive_warp(&ref_set[grp * 4 + (warp & 3)]);
           }
-          if (__any_sync(0xFFFFFFFFu, now != m)) {
+          if (MODE == kShare || __any_sync(0xFFFFFFFFu, moves)) {
             l *= now != m ? exp2_approx(m - now) : 1.0f;
             m = now;
           }
-          if (__any_sync(0xFFFFFFFFu, moves) && j >= (MODE == kSplit ? 2 : 1)) {  // there are sums to bring down
+          if (j >= (MODE == kSplit ? 2 : 1) && __any_sync(0xFFFFFFFFu, moves)) {  // there are sums to bring down
             if (MODE == kShare) {
               if (!hold_warp(sums_done, (done + j - 1u) & 1u, fail)) {
                 ok = false;
@@ -759,12 +782,12 @@ __global__ void __maxnreg__(152)
       if (warp_live && mine > 0) {
         const bool whole = p.t0 == 0 && p.t1 == walk.w.tiles, sees = l > 0.0f || l != l;
         const float inv = sees ? 1.0f / l : 0.0f;
-        const int64_t block = ((int64_t)cta * 2 + (p.t0 == 0)) * a.part_rows + my;
+        const int64_t block = (int64_t)cta * 2 + (p.t0 == 0);
         const unsigned long long fix = odd[k & 1u] & bits;
         constexpr int kCols = MODE == kPair ? DIM : DIM / 2;
         const int c0 = MODE == kPair ? 0 : grp * kCols;
         if (live && (MODE == kPair || grp == 0)) {
-          if (!whole) a.part_stat[block] = make_float2(m - W::kShift, l);
+          if (!whole) a.part_stat[block * a.part_rows + my] = make_float2(m - W::kShift, l);
           else if (a.lse) a.lse[(int64_t)(off + node) * a.Hq + head_q] = sees ? (m - W::kShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
         }
 #pragma unroll 2
@@ -796,20 +819,31 @@ __global__ void __maxnreg__(152)
               }
             }
           }
-          if (live && whole) {
-            char* dst = a.out + (off + node) * a.out_token_stride + head_q * a.out_head_stride + col * 2;
+          if (whole) {
+            // Four lanes hand their rows' 16-byte parts to one another, so that a store writes 64 bytes of a row: one
+            // that writes 16 bytes of 32 rows keeps the store path four times as long.
+            uint4 y[4];
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              uint32_t y[4];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t z[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                y[e] = sees ? W::pack(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv) : 0u;
-              *reinterpret_cast<uint4*>(dst + c * 2) = make_uint4(y[0], y[1], y[2], y[3]);
+              for (int f = 0; f < 4; ++f)
+                z[f] = sees ? W::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv) : 0u;
+              y[e] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+            transpose4(y, lane);
+            const int64_t row_at = (off + node) * a.out_token_stride + head_q * a.out_head_stride + col * 2;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int from = (lane & ~3) + e;
+              const int64_t at = __shfl_sync(0xFFFFFFFFu, row_at, from);
+              if (first_row + (warp & 3) * 32 + from < rows) *reinterpret_cast<uint4*>(a.out + at + (lane & 3) * 16) = y[e];
             }
           } else if (live) {
-            float* dst = a.part + block * DIM + col;
+            float4* dst = a.part + (block * (DIM / 4) + col / 4) * a.part_rows + my;
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            for (int c = 0; c < 32; c += 4)
+              dst[(int64_t)(c / 4) * a.part_rows] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
           }
           __syncwarp();
         }
@@ -920,7 +954,7 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const int c = b + i;
-        const int64_t at = ((int64_t)c * 2 + (c == c0)) * a.part_rows + rr;
+        const int64_t blk = (int64_t)c * 2 + (c == c0);
         unsigned word = pieces[0];
 #pragma unroll
         for (int e = 1; e < (kCtas + 31) / 32; ++e)
@@ -930,11 +964,11 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
 #pragma unroll
         for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
         if (there) {
-          const float* src = a.part + at * DIM + lane * kPer;
-          st[i] = __ldcg(a.part_stat + at);
-          if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+          st[i] = __ldcg(a.part_stat + blk * a.part_rows + rr);
+          const float4* src = a.part + blk * (DIM / 4) * a.part_rows + rr;
+          if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)(lane / 2) * a.part_rows) + lane % 2);
 #pragma unroll
-          for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(reinterpret_cast<const float4*>(src + d));
+          for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(src + (int64_t)(lane * (kPer / 4) + d / 4) * a.part_rows);
         }
       }
       float top = m;
