@@ -112,18 +112,37 @@ int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
+template <typename K>
+cudaError_t ensure_carveout(K kernel, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 template <typename T, int DIM, int MODE>
 int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a, cudaStream_t st) {
   using P = TilePlan<DIM, MODE>;
-  static std::atomic<unsigned long long> attr_done{0};
-  const cudaError_t e = ensure_dynamic_smem(tree_tiles_kernel<T, DIM, MODE>, P::kSmem, attr_done);
+  static std::atomic<unsigned long long> attr_done{0}, room_done{0};
+  cudaError_t e = ensure_dynamic_smem(tree_tiles_kernel<T, DIM, MODE>, P::kSmem, attr_done);
+  // (all of the SM's memory to be shared memory, not as much as this kernel asks for: join_kernel's CTA is to fit beside)
+  if (e == cudaSuccess) e = ensure_carveout(tree_tiles_kernel<T, DIM, MODE>, room_done);
   if (e != cudaSuccess) return set_error(ARCS_ERR_CUDA, cudaGetErrorString(e));
   tree_tiles_kernel<T, DIM, MODE><<<kCtas, kTileThreads, P::kSmem, st>>>(mk, mv, a);
   if (int rc = check_launch("tree_attention")) return rc;
   const int blocks = (a.max_nodes * a.group + P::kRows - 1) / P::kRows;
   const int64_t items = (int64_t)a.c.slots * a.c.heads * blocks;
-  if (items <= kCtas / 2) launch_behind(join_kernel<T, DIM, MODE, 4>, dim3((unsigned)items, (unsigned)a.part_rows), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
-  else launch_behind(join_kernel<T, DIM, MODE, 1>, dim3(kCtas - 1, (unsigned)(a.part_rows + 7) / 8), dim3(kJoinThreads), 0, st, a, kCtas, blocks);
+  int row_bits = 0;
+  while (row_bits < 5 && 1 << row_bits < a.part_rows) ++row_bits;
+  const unsigned groups = (unsigned)((a.part_rows + (1 << row_bits) - 1) >> row_bits);
+  if (items <= kCtas / 2)
+    launch_behind(join_kernel<T, DIM, MODE, true>, dim3((unsigned)items, groups * JoinPlan<DIM, true>::kParts), dim3(kJoinThreads), 0, st, a, kCtas, blocks, row_bits);
+  else
+    launch_behind(join_kernel<T, DIM, MODE, false>, dim3(kCtas - 1, groups * JoinPlan<DIM, false>::kParts), dim3(kJoinThreads), 0, st, a, kCtas, blocks, row_bits);
   return check_launch("tree_attention");
 }
 

@@ -862,24 +862,31 @@ __global__ void __maxnreg__(152)
   if (warp == 9) tmem_free(tmem, 512);
 }
 
-// The pieces of items that were cut, joined. WARPS = 4, for few items of maybe a hundred pieces each:
-// blockIdx.x is the item (slot, key head, block), and four warps work on one row. WARPS = 1, for many:
-// every item that is cut begins in one CTA and goes on in the next, so blockIdx.x names the CTA in
-// which it begins, and a warp takes a row. A warp asks for some pieces' sums at a time, their statistics
-// beside them. Small enough (56 registers, 128 threads) to be on the SM, its way found, while the last
-// pieces are still worked on.
+// The pieces of items that were cut, joined. FEW: few items of maybe a hundred pieces each; blockIdx.x is
+// the item (slot, key head, block). Else many: every item that is cut begins in one CTA and goes on in the
+// next, so blockIdx.x names the CTA in which it begins. A warp takes kCols x 4 columns of 2^row_bits rows
+// (blockIdx.y): as the pieces lie, a lane a row, and where the rows are fewer than the lanes, these
+// share a row's pieces (FEW: the four warps do, too). It asks for some pieces at a time, their statistics
+// beside them: what bounds it is the latency of one such round, 1.7 us for pieces that other SMs have just
+// written. Small enough
+// (56 registers, 128 threads) to be on the SM, its way found, while the last pieces are still worked on.
 constexpr int kJoinThreads = 128;
-template <typename T, int DIM, int MODE, int WARPS>
-__global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, int ctas, int blocks) {
+template <int DIM, bool FEW>
+struct JoinPlan {
+  static constexpr int kCols = FEW ? 1 : 4;                   // of four values each
+  static constexpr int kAtOnce = FEW ? 5 : 2;                 // pieces
+  static constexpr int kParts = DIM / 4 / kCols / (FEW ? 1 : 4);  // CTAs for a group of rows
+};
+template <typename T, int DIM, int MODE, bool FEW>
+__global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, int ctas, int blocks, int row_bits) {
   using P = TilePlan<DIM, MODE>;
   using W = Weight<T>;
-  constexpr int kPer = DIM / 32;
-  __shared__ float2 s_stat[4];
-  __shared__ float s_sum[WARPS == 4 ? 4 : 1][WARPS == 4 ? DIM : 1];
+  using J = JoinPlan<DIM, FEW>;
+  constexpr int kCols = J::kCols;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t total = 0, base = 0, u = 0;
-  int s = WARPS == 4 ? (int)blockIdx.x / (a.c.heads * blocks) : -1, extra = 0;
-  const bool few = WARPS == 4 || a.c.slots <= 128;  // (few items are of few slots)
+  int s = FEW ? (int)blockIdx.x / (a.c.heads * blocks) : -1, extra = 0;
+  const bool few = FEW || a.c.slots <= 128;  // (few items are of few slots)
   if (few) {
     SlotWork w[4];
     uint32_t before[4], own[4];
@@ -887,7 +894,7 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     u = first_unit(total, (int)blockIdx.x + 1, ctas);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool mine = WARPS == 4 ? i * 32 + lane == s : before[i] <= u && u < before[i] + own[i];
+      const bool mine = FEW ? i * 32 + lane == s : before[i] <= u && u < before[i] + own[i];
       const unsigned hit = __ballot_sync(0xFFFFFFFFu, mine);
       if (hit) {
         s = i * 32 + __ffs((int)hit) - 1;
@@ -912,12 +919,12 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
   }
   // (every CTA waits before it ends: what follows on the stream begins when this grid is done, and must not
   // find the tiles still at work)
-  if (s < 0 || (WARPS == 1 && u >= total)) return pdl_wait();
+  if (s < 0 || (!FEW && u >= total)) return pdl_wait();
   const SlotWork w = slot_work<P>(a, s);
   if (w.n == 0) return pdl_wait();
   const Costs<P> costs(a, w, extra);
   int x = (int)(u - base);
-  if (WARPS == 4) {
+  if (FEW) {
     const int i = (int)blockIdx.x - s * a.c.heads * blocks, head = i / blocks;
     if (i - head * blocks >= w.blocks) return pdl_wait();
     x = head * costs.head + (i - head * blocks) * costs.first;
@@ -926,7 +933,7 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
   const int head = at.head, block = at.block;
   const uint32_t tile0 = at.begins + (uint32_t)extra;  // where the item's first tile begins
   const int c0 = cta_of_unit(total, tile0, ctas), c1 = cta_of_unit(total, tile0 + (uint32_t)((w.tiles - 1) * at.cost), ctas);
-  if (c0 == c1 || (WARPS == 1 && c0 != (int)blockIdx.x)) return pdl_wait();  // not cut, or cut before
+  if (c0 == c1 || (!FEW && c0 != (int)blockIdx.x)) return pdl_wait();  // not cut, or cut before
   // CTA c0 + 32 i + lane has a tile of the item: bit `lane` of pieces[i] (with hardly more units than CTAs
   // some of them have none)
   unsigned pieces[(kCtas + 31) / 32];
@@ -942,80 +949,107 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     pieces[i] = __ballot_sync(0xFFFFFFFFu, has);
   }
   const int rows = min(P::kRows, w.n * a.group - block * P::kRows);
+  const int rr = ((int)blockIdx.y / J::kParts << row_bits) + (lane & ((1 << row_bits) - 1));
+  const int share = FEW ? (lane >> row_bits) * 4 + warp : lane >> row_bits, shares = (32 >> row_bits) * (FEW ? 4 : 1);
+  const int col = FEW ? (int)blockIdx.y % J::kParts : ((int)blockIdx.y % J::kParts * 4 + warp) * kCols;  // in steps of four values
+  const bool live = rr < rows;
   if (few) pdl_wait();
-  for (int rr = (int)blockIdx.y * (4 / WARPS) + (WARPS == 4 ? 0 : warp); rr < rows; rr += (int)gridDim.y * (4 / WARPS)) {
-    float m = -INFINITY, l = 0.0f, o[kPer];
+  float m = -INFINITY, l = 0.0f, o[kCols][4];
 #pragma unroll
-    for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
-    constexpr int kAtOnce = DIM == 256 ? 3 : 5;
-    for (int b = c0 + (WARPS == 4 ? warp : 0) * kAtOnce; b <= c1; b += kAtOnce * WARPS) {
-      float y[kAtOnce][kPer];
-      float2 st[kAtOnce];
+  for (int d = 0; d < kCols; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+  for (int b = c0 + share; b <= c1; b += J::kAtOnce * shares) {
+    float4 y[J::kAtOnce][kCols];
+    float2 st[J::kAtOnce];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const int c = b + i;
-        const int64_t blk = (int64_t)c * 2 + (c == c0);
-        unsigned word = pieces[0];
+    for (int i = 0; i < J::kAtOnce; ++i) {
+      const int c = b + i * shares;
+      unsigned word = pieces[0];
 #pragma unroll
-        for (int e = 1; e < (kCtas + 31) / 32; ++e)
-          if ((c - c0) >> 5 == e) word = pieces[e];
-        const bool there = c <= c1 && ((word >> ((c - c0) & 31)) & 1u);
-        st[i] = make_float2(-INFINITY, 0.0f);
+      for (int e = 1; e < (kCtas + 31) / 32; ++e)
+        if ((c - c0) >> 5 == e) word = pieces[e];
+      const bool there = live && c <= c1 && ((word >> ((c - c0) & 31)) & 1u);
+      const int64_t blk = (int64_t)c * 2 + (c == c0);
+      st[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) y[i][d] = 0.0f;
-        if (there) {
-          st[i] = __ldcg(a.part_stat + blk * a.part_rows + rr);
-          const float4* src = a.part + blk * (DIM / 4) * a.part_rows + rr;
-          if (kPer == 2) *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)(lane / 2) * a.part_rows) + lane % 2);
+      for (int d = 0; d < kCols; ++d) y[i][d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (there) {
+        st[i] = __ldcg(a.part_stat + blk * a.part_rows + rr);
 #pragma unroll
-          for (int d = 0; d + 3 < kPer; d += 4) *reinterpret_cast<float4*>(y[i] + d) = __ldcg(src + (int64_t)(lane * (kPer / 4) + d / 4) * a.part_rows);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
-      const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
-      m = top;
-      l = weighed(f, l);
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) o[d] = weighed(f, o[d]);
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const float wt = exp2_approx(st[i].x - ref);
-        l += wt * st[i].y;
-#pragma unroll
-        for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, y[i][d]);
+        for (int d = 0; d < kCols; ++d) y[i][d] = __ldcg(a.part + (blk * (DIM / 4) + col + d) * a.part_rows + rr);
       }
     }
-    if (WARPS == 4) {  // the four warps' shares
-      if (lane == 0) s_stat[warp] = make_float2(m, l);
+    float top = m;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) s_sum[warp][lane * kPer + d] = o[d];
-      __syncthreads();
-      m = fmaxf(fmaxf(s_stat[0].x, s_stat[1].x), fmaxf(s_stat[2].x, s_stat[3].x));
-      const float ref = m == -INFINITY ? 0.0f : m;
-      l = 0.0f;
+    for (int i = 0; i < J::kAtOnce; ++i) top = fmaxf(top, st[i].x);
+    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    m = top;
+    l = weighed(f, l);
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) o[d] = 0.0f;
+    for (int d = 0; d < kCols; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float wt = exp2_approx(s_stat[i].x - ref);
-        l += weighed(wt, s_stat[i].y);
+      for (int e = 0; e < 4; ++e) o[d][e] = weighed(f, o[d][e]);
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) o[d] += weighed(wt, s_sum[i][lane * kPer + d]);
+    for (int i = 0; i < J::kAtOnce; ++i) {
+      const float wt = exp2_approx(st[i].x - ref);
+      l += weighed(wt, st[i].y);
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) {
+        o[d][0] += weighed(wt, y[i][d].x);
+        o[d][1] += weighed(wt, y[i][d].y);
+        o[d][2] += weighed(wt, y[i][d].z);
+        o[d][3] += weighed(wt, y[i][d].w);
       }
-      __syncthreads();
-    }
-    if (WARPS == 1 || warp == 0) {
-      const bool sees = l > 0.0f || l != l;
-      const float inv = sees ? 1.0f / l : 0.0f;
-      const int x = block * P::kRows + rr, node = x / a.group, h = head * a.group + x - node * a.group;
-      char* dst = a.out + (w.off + node) * a.out_token_stride + h * a.out_head_stride + lane * kPer * 2;
-#pragma unroll
-      for (int d = 0; d < kPer; d += 2) *reinterpret_cast<uint32_t*>(dst + d * 2) = sees ? W::pack(o[d] * inv, o[d + 1] * inv) : 0u;
-      if (a.lse && lane == 0) a.lse[(int64_t)(w.off + node) * a.Hq + h] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
   }
+  for (int x = 16; x >= 1 << row_bits; x >>= 1) {  // the lanes' shares of a row
+    const float top = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)), ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    m = top;
+    l = weighed(f, l);
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+#pragma unroll
+    for (int d = 0; d < kCols; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[d][e] = weighed(f, o[d][e]);
+        o[d][e] += __shfl_xor_sync(0xFFFFFFFFu, o[d][e], x);
+      }
+  }
+  if (FEW) {  // the warps'
+    __shared__ float meet[3][6][32];
+    if (warp > 0) {
+      float* mine = &meet[warp - 1][0][lane];
+      mine[0] = m;
+      mine[32] = l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[64 + 32 * e] = o[0][e];
+    }
+    __syncthreads();
+    if (warp > 0) return;
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) top = fmaxf(top, meet[i][0][lane]);
+    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    m = top;
+    l = weighed(f, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[0][e] = weighed(f, o[0][e]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const float wt = exp2_approx(meet[i][0][lane] - ref);
+      l += weighed(wt, meet[i][1][lane]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[0][e] += weighed(wt, meet[i][2 + e][lane]);
+    }
+  }
+  if (!live || lane >> row_bits) return;
+  const bool sees = l > 0.0f || l != l;
+  const float inv = sees ? 1.0f / l : 0.0f;
+  const int row = block * P::kRows + rr, node = row / a.group, h = head * a.group + row - node * a.group;
+  char* dst = a.out + (w.off + node) * a.out_token_stride + h * a.out_head_stride + col * 8;
+#pragma unroll
+  for (int d = 0; d < kCols; ++d)
+    *reinterpret_cast<uint2*>(dst + d * 8) = sees ? make_uint2(W::pack(o[d][0] * inv, o[d][1] * inv), W::pack(o[d][2] * inv, o[d][3] * inv)) : make_uint2(0u, 0u);
+  if (a.lse && col == 0) a.lse[(int64_t)(w.off + node) * a.Hq + h] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 }  // namespace arcs
