@@ -40,9 +40,9 @@ struct TilePlan {
   static constexpr int kSub = DIM == 256 ? 2 : 1;
   static constexpr int kQBytes = kRows * DIM * 2;
   static constexpr int kTile = kKeys * DIM * 2 / kSub;         // 32 KB, at dim 64 16 KB
-  // slots of the ring: 128 to 160 KB a CTA keep the memory busy (20 MB under way on all of them). kSplit
-  // and kShare leave room beside them for a CTA of join_kernel.
-  static constexpr int kSlots = DIM == 64 ? 10 : MODE == kShare ? 4 : 5;
+  // slots of the ring: 160 KB a CTA keep the memory busy (24 MB under way on all of them). kSplit leaves room
+  // beside them for a CTA of join_kernel; at dim 256 a fifth slot gains more (84 -> 79 us for 24 nodes over 131071).
+  static constexpr int kSlots = DIM == 64 ? 10 : 5;
   static constexpr int kSmem = kQBytes + kSlots * kTile + 2048 + 1024;
   static constexpr uint32_t kScore1 = kKeys;                   // columns: scores 0, scores 1, sums from 256 on
   static constexpr uint32_t kSums = 256;
@@ -237,8 +237,8 @@ __device__ __forceinline__ void transpose4(uint4 (&y)[4], int lane) {
   }
 }
 
-// weight * sum, where the weight may have been rounded to nothing and the sum may be infinite
-__device__ __forceinline__ float weighed(float w, float o) { return w == 0.0f ? (fabsf(o) <= 3.402823466e38f ? 0.0f : o) : w * o; }
+// 2^x, but never nothing: what it weighs may be infinite, and a finite sum times this is nothing anyway
+__device__ __forceinline__ float weight_of(float x) { return fmaxf(exp2_approx(x), 1.17549435e-38f); }
 
 // Up to 128 slots, a warp on its own: four slots a lane, the units before each, and the units in all.
 template <typename P>
@@ -775,13 +775,15 @@ __global__ void __maxnreg__(152)
         const float2 s0 = stat[row_t], s1 = stat[128 + row_t];
         m = fmaxf(s0.x, s1.x);
         const float ref = m == -INFINITY ? 0.0f : m;
-        f0 = exp2_approx(s0.x - ref);
-        f1 = exp2_approx(s1.x - ref);
+        f0 = weight_of(s0.x - ref);
+        f1 = weight_of(s1.x - ref);
         l = f0 * s0.y + f1 * s1.y;
       }
       if (warp_live && mine > 0) {
         const bool whole = p.t0 == 0 && p.t1 == walk.w.tiles, sees = l > 0.0f || l != l;
-        const float inv = sees ? 1.0f / l : 0.0f;
+        const float inv = !whole ? 1.0f : sees ? 1.0f / l : 0.0f;
+        if (MODE != kSplit) f0 = 1.0f;  // (kShare: the sums are those of both groups)
+        const uint64_t g0 = pair_of(f0 * inv, f0 * inv), g1 = pair_of(f1 * inv, f1 * inv);
         const int64_t block = (int64_t)cta * 2 + (p.t0 == 0);
         const unsigned long long fix = odd[k & 1u] & bits;
         constexpr int kCols = MODE == kPair ? DIM : DIM / 2;
@@ -795,17 +797,30 @@ __global__ void __maxnreg__(152)
           const int col = c0 + i * 32;
           uint32_t o[32];
           tmem_ld32(o, lanes + P::kSums + (MODE == kPair ? grp * DIM : 0) + col);
-          if (MODE == kSplit && n > 1) {  // (with one tile the other group has no sums, and f0 is 1 or the row saw nothing)
+          if (MODE == kSplit && n > 1) {  // (with one tile the other group has no sums)
             uint32_t o1[32];
             tmem_ld32(o1, lanes + P::kSums + DIM + col);
             tmem_wait_ld();
             tmem_use(o);
             tmem_use(o1);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(weighed(f0, __uint_as_float(o[c])) + weighed(f1, __uint_as_float(o1[c])));
+            for (int c = 0; c < 32; c += 2) {
+              float y0, y1;
+              pair_out(fma_pair(pair_of(__uint_as_float(o1[c]), __uint_as_float(o1[c + 1])), g1, mul_pair(pair_of(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), g0)), y0, y1);
+              o[c] = __float_as_uint(y0);
+              o[c + 1] = __float_as_uint(y1);
+            }
+          } else {
+            tmem_wait_ld();
+            tmem_use(o);
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float y0, y1;
+              pair_out(mul_pair(pair_of(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), g0), y0, y1);
+              o[c] = __float_as_uint(y0);
+              o[c + 1] = __float_as_uint(y1);
+            }
           }
-          tmem_wait_ld();
-          tmem_use(o);
           if (fix) {
             for (unsigned long long f = fix; f; f &= f - 1) {
               const int place = len + __ffsll((long long)f) - 1, pg = a.c.table[(int64_t)walk.s * a.c.max_pages + (place >> a.c.page_shift)];
@@ -828,7 +843,7 @@ __global__ void __maxnreg__(152)
               uint32_t z[4];
 #pragma unroll
               for (int f = 0; f < 4; ++f)
-                z[f] = sees ? W::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv) : 0u;
+                z[f] = sees ? W::pack(__uint_as_float(o[8 * e + 2 * f]), __uint_as_float(o[8 * e + 2 * f + 1])) : 0u;
               y[e] = make_uint4(z[0], z[1], z[2], z[3]);
             }
             transpose4(y, lane);
@@ -981,36 +996,36 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     float top = m;
 #pragma unroll
     for (int i = 0; i < J::kAtOnce; ++i) top = fmaxf(top, st[i].x);
-    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    const float ref = top == -INFINITY ? 0.0f : top, f = weight_of(m - ref);
     m = top;
-    l = weighed(f, l);
+    l = f * l;
 #pragma unroll
     for (int d = 0; d < kCols; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[d][e] = weighed(f, o[d][e]);
+      for (int e = 0; e < 4; ++e) o[d][e] = f * o[d][e];
 #pragma unroll
     for (int i = 0; i < J::kAtOnce; ++i) {
-      const float wt = exp2_approx(st[i].x - ref);
-      l += weighed(wt, st[i].y);
+      const float wt = weight_of(st[i].x - ref);
+      l += wt * st[i].y;
 #pragma unroll
       for (int d = 0; d < kCols; ++d) {
-        o[d][0] += weighed(wt, y[i][d].x);
-        o[d][1] += weighed(wt, y[i][d].y);
-        o[d][2] += weighed(wt, y[i][d].z);
-        o[d][3] += weighed(wt, y[i][d].w);
+        o[d][0] += wt * y[i][d].x;
+        o[d][1] += wt * y[i][d].y;
+        o[d][2] += wt * y[i][d].z;
+        o[d][3] += wt * y[i][d].w;
       }
     }
   }
   for (int x = 16; x >= 1 << row_bits; x >>= 1) {  // the lanes' shares of a row
-    const float top = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)), ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    const float top = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)), ref = top == -INFINITY ? 0.0f : top, f = weight_of(m - ref);
     m = top;
-    l = weighed(f, l);
+    l = f * l;
     l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
 #pragma unroll
     for (int d = 0; d < kCols; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        o[d][e] = weighed(f, o[d][e]);
+        o[d][e] = f * o[d][e];
         o[d][e] += __shfl_xor_sync(0xFFFFFFFFu, o[d][e], x);
       }
   }
@@ -1028,17 +1043,17 @@ __global__ void __launch_bounds__(kJoinThreads, 9) join_kernel(const TreeDev a, 
     float top = m;
 #pragma unroll
     for (int i = 0; i < 3; ++i) top = fmaxf(top, meet[i][0][lane]);
-    const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(m - ref);
+    const float ref = top == -INFINITY ? 0.0f : top, f = weight_of(m - ref);
     m = top;
-    l = weighed(f, l);
+    l = f * l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[0][e] = weighed(f, o[0][e]);
+    for (int e = 0; e < 4; ++e) o[0][e] = f * o[0][e];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const float wt = exp2_approx(meet[i][0][lane] - ref);
-      l += weighed(wt, meet[i][1][lane]);
+      const float wt = weight_of(meet[i][0][lane] - ref);
+      l += wt * meet[i][1][lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[0][e] += weighed(wt, meet[i][2 + e][lane]);
+      for (int e = 0; e < 4; ++e) o[0][e] += wt * meet[i][2 + e][lane];
     }
   }
   if (!live || lane >> row_bits) return;
