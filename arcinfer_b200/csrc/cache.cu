@@ -406,43 +406,36 @@ template <> struct Half2Of<__half> {
   }
 };
 
-// A CTA takes `per` rows (up to four: with many rows the way to a row's place, four dependent trips to memory,
-// is what bounds a CTA with one). Four warps find the places, the others the turns of the rotation, once
-// for all heads: in fp64, pos * inv_freq / 2 pi less its whole part, so that a position of any size
-// leaves an angle exact to fp32. Meanwhile the first heads are on their way: a head is DIM / 8 neighbouring
-// lanes with 16 bytes each, and a lane's next kAhead heads are always asked for. What bounds it then is
-// the memory: each value once in and once out.
+// A CTA takes ROWS rows (four where there are many: the way to a row's place, four dependent trips to memory,
+// is what bounds a CTA with one). A head is DIM / 8 neighbouring lanes with 16 bytes each; a lane
+// stays with a head for all rows, so that weights and addresses are found once, and its next head's rows
+// are always asked for. Meanwhile, at the start, a warp a row finds the place, and the others the turns of
+// the rotation, once for all heads: in fp64, pos * inv_freq / 2 pi less its whole part, so that a
+// position of any size leaves an angle exact to fp32. What bounds it is the memory, each value once in
+// and once out, and hardly less the instructions: some 150 for 16 bytes.
 constexpr int kAppendRows = 4;
-template <typename T, int DIM>
-__global__ void __launch_bounds__(256, 5) append_kernel(const AppendDev a, int per) {
-  __shared__ float2 turn[kAppendRows][DIM / 2];
-  __shared__ int64_t s_at[kAppendRows];  // bytes into a head of the layer; -1: nowhere, -2: not even the query
-  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes, kAhead = 3;
-  const int t0 = blockIdx.x * per, rows = min(per, a.T - t0), tid = threadIdx.x;
+template <typename T, int DIM, int ROWS>
+__global__ void __launch_bounds__(256, ROWS == 1 ? 5 : 4) append_kernel(const AppendDev a) {
+  __shared__ float2 turn[ROWS][DIM / 2];
+  __shared__ int64_t s_at[ROWS];  // bytes into a head of the layer; -1: nowhere, -2: not even the query
+  constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes;
+  const int t0 = blockIdx.x * ROWS, rows = min(ROWS, a.T - t0), tid = threadIdx.x;
   const int lane = tid % kLanes, e0 = lane * 8, all = a.Hq + 2 * a.c.heads, half = a.rot / 2;
-  struct At {  // a row of this CTA's and a head of it
-    int r, g;
-  };
-  auto forward = [&](At& p) {
-    for (p.g += kGroups; p.g >= all; p.g -= all) ++p.r;
-  };
-  auto load = [&](const At& p) {
-    const int64_t t = t0 + p.r;
-    const char* src = p.g < a.Hq ? a.q + t * a.q_stride : p.g < a.Hq + a.c.heads ? a.k + t * a.k_stride : a.v + t * a.v_stride;
-    const int h = p.g < a.Hq ? p.g : p.g < a.Hq + a.c.heads ? p.g - a.Hq : p.g - a.Hq - a.c.heads;
-    return *reinterpret_cast<const uint4*>(src + h * (DIM * 2) + lane * 16);
-  };
-  uint4 ahead[kAhead];
-  At now{0, tid / kLanes - kGroups}, next;
-  forward(now);
-  next = now;
+  auto load = [&](int g, uint4 (&x)[ROWS]) {
+    const bool is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
+    const int64_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
+    const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
+    const char* src = (is_q ? a.q : is_v ? a.v : a.k) + t0 * stride + h * (DIM * 2) + lane * 16;
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    ahead[i] = make_uint4(0, 0, 0, 0);
-    if (next.r < rows) ahead[i] = load(next);
-    forward(next);
-  }
-  if (tid < 32 * kAppendRows) {
+    for (int r = 0; r < ROWS; ++r) {
+      x[r] = make_uint4(0, 0, 0, 0);
+      if (g < all && r < rows) x[r] = *reinterpret_cast<const uint4*>(src);
+      src += stride;
+    }
+  };
+  uint4 ahead[ROWS];
+  load(tid / kLanes, ahead);
+  if (tid < 32 * ROWS) {
     const int r = tid / 32;
     if (r < rows) {
       const int t = t0 + r, s = slot_of_row(a.node_off, a.c.slots, t);
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendDev a, int p
       }
     }
   } else if (half > 0) {
-    for (int i = tid - 32 * kAppendRows; i < rows * half; i += 256 - 32 * kAppendRows) {
+    for (int i = tid - 32 * ROWS; i < rows * half; i += 256 - 32 * ROWS) {
       const int r = i / half, e = i - r * half;
       const double turns = (double)a.pos[t0 + r] * a.inv_freq[e] * 0.15915494309189533577;
       float sn, cs;
@@ -472,49 +465,54 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendDev a, int p
     }
   }
   __syncthreads();
-  // (the lanes of a warp may be at different heads, but all go on until the last of them has none)
-  while (__any_sync(0xFFFFFFFFu, now.r < rows)) {
+  for (int g0 = 0; g0 < all; g0 += kGroups) {
+    const int g = g0 + tid / kLanes;
+    const bool is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads, live = g < all;
+    const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
+    uint4 x[ROWS];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const bool live = now.r < rows, is_q = now.g < a.Hq, is_v = now.g >= a.Hq + a.c.heads;
-      const int h = is_q ? now.g : is_v ? now.g - a.Hq - a.c.heads : now.g - a.Hq;
-      uint4 x = ahead[i];
-      if (next.r < rows) ahead[i] = load(next);
-      forward(next);
-      if (!__all_sync(0xFFFFFFFFu, is_v || !live)) {
+    for (int r = 0; r < ROWS; ++r) x[r] = ahead[r];
+    load(g + kGroups, ahead);
+    const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+    const bool norms = a.q_weight || a.k_weight, copied = __all_sync(0xFFFFFFFFu, is_v || !live);
+    float4 w0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w1 = w0;
+    if (w && live) {
+      w0 = __ldg(reinterpret_cast<const float4*>(w + e0));
+      w1 = __ldg(reinterpret_cast<const float4*>(w + e0) + 1);
+    }
+    char* dst = is_q ? a.q_out + t0 * a.q_out_stride + h * (DIM * 2) + lane * 16 : (is_v ? a.c.v : a.c.k) + h * a.c.head_stride + lane * 16;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (r >= rows) break;
+      if (!copied) {
         float y[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 f = Half2Of<T>::widen(j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w);
+          const float2 f = Half2Of<T>::widen(j == 0 ? x[r].x : j == 1 ? x[r].y : j == 2 ? x[r].z : x[r].w);
           y[2 * j] = f.x;
           y[2 * j + 1] = f.y;
         }
-        const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
-        if (a.q_weight || a.k_weight) {
+        if (norms) {
           float ss = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-          if (w && live) {
-            const float r = rsqrtf(ss * (1.0f / DIM) + a.eps);
-            const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + e0)), w1 = __ldg(reinterpret_cast<const float4*>(w + e0) + 1);
-            y[0] *= r * w0.x;
-            y[1] *= r * w0.y;
-            y[2] *= r * w0.z;
-            y[3] *= r * w0.w;
-            y[4] *= r * w1.x;
-            y[5] *= r * w1.y;
-            y[6] *= r * w1.z;
-            y[7] *= r * w1.w;
-          }
+          const float n = w ? rsqrtf(ss * (1.0f / DIM) + a.eps) : 1.0f;
+          y[0] *= n * w0.x;
+          y[1] *= n * w0.y;
+          y[2] *= n * w0.z;
+          y[3] *= n * w0.w;
+          y[4] *= n * w1.x;
+          y[5] *= n * w1.y;
+          y[6] *= n * w1.z;
+          y[7] *= n * w1.w;
         }
-        const float2* turns = turn[live ? now.r : 0];
         if (a.interleaved) {
           if (e0 < a.rot) {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-              const float2 f = turns[(e0 + j) / 2];
+              const float2 f = turn[r][(e0 + j) / 2];
               const float u = y[j] * f.x - y[j + 1] * f.y;
               y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
               y[j] = u;
@@ -528,21 +526,17 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendDev a, int p
           for (int j = 0; j < 8; ++j) {
             const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
             if (e0 < a.rot) {
-              const float2 f = turns[(first ? e0 : e0 - half) + j];
+              const float2 f = turn[r][(first ? e0 : e0 - half) + j];
               y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
             }
           }
         }
-        if (!is_v) x = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
+        if (!is_v) x[r] = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
       }
       if (live) {
-        const int64_t at = s_at[now.r];
-        if (at >= (is_q ? -1 : 0)) {
-          char* dst = is_q ? a.q_out + (t0 + now.r) * a.q_out_stride + h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + at + h * a.c.head_stride;
-          *reinterpret_cast<uint4*>(dst + lane * 16) = x;
-        }
+        const int64_t at = s_at[r];
+        if (at >= (is_q ? -1 : 0)) *reinterpret_cast<uint4*>(dst + (is_q ? r * a.q_out_stride : at)) = x[r];
       }
-      forward(now);
     }
   }
 }
@@ -636,18 +630,24 @@ extern "C" int arcs_cache_append(const arcs_append_args* g, void* stream) {
   a.pos = g->pos;
   a.node_off = g->node_off;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // (rows enough to give every SM its five CTAs of four rows: then four. 500 rows took ? us with one, ? with four;
+  // (rows enough to give every SM its four CTAs of four rows: then four. 500 rows took ? us with one, ? with four;
   // 14,700 rows ? and ? us)
-  const int per = g->T >= kSmCount * 5 * kAppendRows ? kAppendRows : 1;
-  const unsigned grid = (unsigned)((g->T + per - 1) / per);
-#define ARCS_LAUNCH(TYPE)                                                     \
-  do {                                                                        \
-    if (c->dim == 64) append_kernel<TYPE, 64><<<grid, 256, 0, st>>>(a, per);       \
-    else if (c->dim == 128) append_kernel<TYPE, 128><<<grid, 256, 0, st>>>(a, per); \
-    else append_kernel<TYPE, 256><<<grid, 256, 0, st>>>(a, per);                   \
+  const bool many = g->T >= kSmCount * 4 * kAppendRows;
+  const unsigned grid = (unsigned)(many ? (g->T + kAppendRows - 1) / kAppendRows : g->T);
+#define ARCS_ROWS(TYPE, D)                                                                \
+  do {                                                                                    \
+    if (many) append_kernel<TYPE, D, kAppendRows><<<grid, 256, 0, st>>>(a);               \
+    else append_kernel<TYPE, D, 1><<<grid, 256, 0, st>>>(a);                              \
+  } while (0)
+#define ARCS_LAUNCH(TYPE)                        \
+  do {                                           \
+    if (c->dim == 64) ARCS_ROWS(TYPE, 64);       \
+    else if (c->dim == 128) ARCS_ROWS(TYPE, 128); \
+    else ARCS_ROWS(TYPE, 256);                   \
   } while (0)
   if (c->dtype == ARCS_BF16) ARCS_LAUNCH(__nv_bfloat16);
   else ARCS_LAUNCH(__half);
 #undef ARCS_LAUNCH
+#undef ARCS_ROWS
   return check_launch("cache_append");
 }
