@@ -868,7 +868,7 @@ __global__ void __maxnreg__(152)
       arrive_warp(sums_free);
       rc0 += 2 * n * P::kSub;
       done += n;
-      if (MODE == kShare && warp_live && (n & 1) == grp && n > grp) ++set;  // (the piece's last tile was the other group's: nobody asked for its reference)
+      if (MODE == kShare && warp_live && (n & 1) == grp) ++set;  // (the piece's last tile was the other group's: nobody asked for its reference)
       ++k;
     }
   }

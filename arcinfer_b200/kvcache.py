@@ -240,7 +240,8 @@ def accept_tree(token, draft, parent, node_off, max_nodes, status=None):
     dev = token.device
     T, slots = token.numel(), node_off.numel() - 1
     args = (_list("token", token, _i32, None, dev), _list("draft", draft, _i32, T, dev), _list("parent", parent, _i32, T, dev), _list("node_off", node_off, _i32, None, dev))
-    accepted, kept, last = _empty((3, slots), dtype=_i32, device=dev).unbind(0)
+    accepted = _empty(slots, dtype=_i32, device=dev)
+    kept, last = torch.empty_like(accepted), torch.empty_like(accepted)
     path = _empty((slots, max_nodes), dtype=_i32, device=dev)
     _enqueue(dev, lib.arcs_accept_tree, "arcs_accept_tree", *args, slots, T, max_nodes, accepted.data_ptr(), kept.data_ptr(), last.data_ptr(), path.data_ptr(), max_nodes,
              None if status is None else _list("status", status, _i32, 1, dev))

@@ -54,6 +54,39 @@ def test_large_trees(dim, Hq, heads):
     _check(cache, rows, off, masks, q, got, lens)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,Hq,heads,most", [(64, 16, 8, 6), (64, 40, 8, 40), (128, 16, 8, 6), (128, 40, 8, 40), (256, 16, 8, 6), (256, 40, 8, 30)])
+def test_many_short_texts(dim, Hq, heads, most, dtype):
+    """several items, whole and cut, of one tile and of several, for every CTA"""
+    import arcinfer_b200 as ab
+    import kvutil as kv
+
+    g = np.random.default_rng(dim + Hq)
+    slots = 40
+    lens = [int(x) for x in g.choice([0, 3, 100, 120, 129, 250, 300, 380, 500, 640, 900], slots)]
+    nodes = [int(x) for x in g.integers(0, most + 1, slots)]
+    cache, rows, off, masks, mask, q = _case(dim + Hq, lens, nodes, Hq, heads, 32, dim, kv.DTYPES[dtype])
+    for _ in range(3):
+        got = ab.tree_attention(q, cache, kv.i32(off), most, mask=mask, want_lse=True)
+        _check(cache, rows, off, masks, q, got, lens)
+
+
+@pytest.mark.parametrize("slots", [129, 700])
+def test_many_slots(slots):
+    """more slots than a warp adds up on its own"""
+    import arcinfer_b200 as ab
+    import kvutil as kv
+
+    for dim, Hq in ((64, 8), (128, 2), (128, 48), (256, 4)):
+        g = np.random.default_rng(slots + dim)
+        lens = [int(x) for x in g.integers(0, 200, slots)]
+        lens[slots // 2] = 5000
+        nodes = [int(x) for x in g.choice([0, 0, 1, 2, 7], slots)]
+        cache, rows, off, masks, mask, q = _case(dim, lens, nodes, Hq, 2, 16, dim)
+        got = ab.tree_attention(q, cache, kv.i32(off), 7, mask=mask, want_lse=True)
+        _check(cache, rows, off, masks, q, got, lens)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("length", [1, 40, 128, 129, 5000, 40000])
 def test_single_tokens(dim, length):
