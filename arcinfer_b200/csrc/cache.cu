@@ -303,7 +303,7 @@ __device__ __forceinline__ bool follow(const CacheDev& c, int s, int used, int l
 // one (layer, pool, head) at a time: it reads up to eight rows before it writes them, in ascending order,
 // so no row is written before it has been read. The way to the rows is three dependent trips to
 // memory (path, pages, their holders), so a CTA takes as many columns as fill the machine twice
-// over rather than one a thread: 64 slots x 8192 columns took ? us with one, ? with this.
+// over rather than one a thread. 64 slots x 8192 columns x 7 rows: 21.6 us, 5.4 TB/s.
 __global__ void __launch_bounds__(256) compact_move_kernel(const CacheDev c, const int32_t* __restrict__ kept_, const int32_t* __restrict__ path_, int path_stride) {
   pdl_trigger();
   __shared__ int64_t from[ARCS_TREE_MAX], to[ARCS_TREE_MAX];
@@ -407,29 +407,41 @@ template <> struct Half2Of<__half> {
 };
 
 // A CTA takes ROWS rows (four where there are many: the way to a row's place, four dependent trips to memory,
-// is what bounds a CTA with one). A head is DIM / 8 neighbouring lanes with 16 bytes each; a lane
+// is what bounds a CTA with one). A head is DIM / 8 neighbouring lanes with twice four values each; a lane
 // stays with a head for all rows, so that weights and addresses are found once, and its next head's rows
-// are always asked for. Meanwhile, at the start, a warp a row finds the place, and the others the turns of
+// are always asked for. Lane l < rot / 8 has the values 4 l .. and rot / 2 + 4 l .. (interleaved: 8 l ..), so that
+// both of a pair are its own and its turns are 4 l .., the other lanes what is not rotated: with 16 bytes in a
+// row instead, eight shuffles a head brought the pairs together, and 14,700 rows of 48 heads of 128 took
+// 125 us. Meanwhile, at the start, a warp a row finds the place, and the others the turns of
 // the rotation, once for all heads: in fp64, pos * inv_freq / 2 pi less its whole part, so that a
 // position of any size leaves an angle exact to fp32. What bounds it is the memory, each value once in
-// and once out, and hardly less the instructions: some 150 for 16 bytes.
+// and once out, and hardly less the instructions.
 constexpr int kAppendRows = 4;
 template <typename T, int DIM, int ROWS>
 __global__ void __launch_bounds__(256, ROWS == 1 ? 5 : 4) append_kernel(const AppendDev a) {
-  __shared__ float2 turn[ROWS][DIM / 2];
+  __shared__ __align__(16) float2 turn[ROWS][DIM / 2];
   __shared__ int64_t s_at[ROWS];  // bytes into a head of the layer; -1: nowhere, -2: not even the query
   constexpr int kLanes = DIM / 8, kGroups = 256 / kLanes;
   const int t0 = blockIdx.x * ROWS, rows = min(ROWS, a.T - t0), tid = threadIdx.x;
-  const int lane = tid % kLanes, e0 = lane * 8, all = a.Hq + 2 * a.c.heads, half = a.rot / 2;
+  const int lane = tid % kLanes, all = a.Hq + 2 * a.c.heads, half = a.rot / 2;
+  const bool turns_here = lane < a.rot / 8;
+  const int e0 = a.interleaved ? 8 * lane : turns_here ? 4 * lane : a.rot + 8 * (lane - a.rot / 8), e1 = a.interleaved || !turns_here ? e0 + 4 : half + 4 * lane;
   auto load = [&](int g, uint4 (&x)[ROWS]) {
     const bool is_q = g < a.Hq, is_v = g >= a.Hq + a.c.heads;
     const int64_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
     const int h = is_q ? g : is_v ? g - a.Hq - a.c.heads : g - a.Hq;
-    const char* src = (is_q ? a.q : is_v ? a.v : a.k) + t0 * stride + h * (DIM * 2) + lane * 16;
+    const char* src = (is_q ? a.q : is_v ? a.v : a.k) + t0 * stride + h * (DIM * 2);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       x[r] = make_uint4(0, 0, 0, 0);
-      if (g < all && r < rows) x[r] = *reinterpret_cast<const uint4*>(src);
+      if (g < all && r < rows) {
+        if (a.interleaved) {
+          x[r] = *reinterpret_cast<const uint4*>(src + e0 * 2);
+        } else {
+          const uint2 lo = *reinterpret_cast<const uint2*>(src + e0 * 2), hi = *reinterpret_cast<const uint2*>(src + e1 * 2);
+          x[r] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
       src += stride;
     }
   };
@@ -478,9 +490,9 @@ __global__ void __launch_bounds__(256, ROWS == 1 ? 5 : 4) append_kernel(const Ap
     float4 w0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w1 = w0;
     if (w && live) {
       w0 = __ldg(reinterpret_cast<const float4*>(w + e0));
-      w1 = __ldg(reinterpret_cast<const float4*>(w + e0) + 1);
+      w1 = __ldg(reinterpret_cast<const float4*>(w + e1));
     }
-    char* dst = is_q ? a.q_out + t0 * a.q_out_stride + h * (DIM * 2) + lane * 16 : (is_v ? a.c.v : a.c.k) + h * a.c.head_stride + lane * 16;
+    char* dst = is_q ? a.q_out + t0 * a.q_out_stride + h * (DIM * 2) : (is_v ? a.c.v : a.c.k) + h * a.c.head_stride;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       if (r >= rows) break;
@@ -508,34 +520,38 @@ __global__ void __launch_bounds__(256, ROWS == 1 ? 5 : 4) append_kernel(const Ap
           y[6] *= n * w1.z;
           y[7] *= n * w1.w;
         }
-        if (a.interleaved) {
-          if (e0 < a.rot) {
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const float2 f = turn[r][(e0 + j) / 2];
-              const float u = y[j] * f.x - y[j + 1] * f.y;
-              y[j + 1] = y[j] * f.y + y[j + 1] * f.x;
-              y[j] = u;
-            }
-          }
-        } else if (a.rot) {
-          // the pair's other value is in the lane rot / 16 further, or before
-          const bool first = e0 < half;
-          const int other = first ? lane + half / 8 : e0 < a.rot ? lane - half / 8 : lane;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float z = __shfl_sync(0xFFFFFFFFu, y[j], other, kLanes);
-            if (e0 < a.rot) {
-              const float2 f = turn[r][(first ? e0 : e0 - half) + j];
-              y[j] = first ? y[j] * f.x - z * f.y : z * f.y + y[j] * f.x;
-            }
+        if (turns_here) {
+          const float4 f0 = *reinterpret_cast<const float4*>(&turn[r][4 * lane]), f1 = *reinterpret_cast<const float4*>(&turn[r][4 * lane + 2]);
+          auto rotate = [](float& u, float& v, float c, float s) {
+            const float w = u * c - v * s;
+            v = u * s + v * c;
+            u = w;
+          };
+          if (a.interleaved) {
+            rotate(y[0], y[1], f0.x, f0.y);
+            rotate(y[2], y[3], f0.z, f0.w);
+            rotate(y[4], y[5], f1.x, f1.y);
+            rotate(y[6], y[7], f1.z, f1.w);
+          } else {
+            rotate(y[0], y[4], f0.x, f0.y);
+            rotate(y[1], y[5], f0.z, f0.w);
+            rotate(y[2], y[6], f1.x, f1.y);
+            rotate(y[3], y[7], f1.z, f1.w);
           }
         }
         if (!is_v) x[r] = make_uint4(Half2Of<T>::pack(y[0], y[1]), Half2Of<T>::pack(y[2], y[3]), Half2Of<T>::pack(y[4], y[5]), Half2Of<T>::pack(y[6], y[7]));
       }
       if (live) {
         const int64_t at = s_at[r];
-        if (at >= (is_q ? -1 : 0)) *reinterpret_cast<uint4*>(dst + (is_q ? r * a.q_out_stride : at)) = x[r];
+        if (at >= (is_q ? -1 : 0)) {
+          char* to = dst + (is_q ? r * a.q_out_stride : at);
+          if (a.interleaved) {
+            *reinterpret_cast<uint4*>(to + e0 * 2) = x[r];
+          } else {
+            *reinterpret_cast<uint2*>(to + e0 * 2) = make_uint2(x[r].x, x[r].y);
+            *reinterpret_cast<uint2*>(to + e1 * 2) = make_uint2(x[r].z, x[r].w);
+          }
+        }
       }
     }
   }
@@ -630,9 +646,9 @@ extern "C" int arcs_cache_append(const arcs_append_args* g, void* stream) {
   a.pos = g->pos;
   a.node_off = g->node_off;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // (rows enough to give every SM its four CTAs of four rows: then four. 500 rows took ? us with one, ? with four;
-  // 14,700 rows ? and ? us)
-  const bool many = g->T >= kSmCount * 4 * kAppendRows;
+  // (four rows a CTA where all SMs have their four CTAs of four rows one and a half times over: of 48 heads of 128, 500 rows took 6.2 us with one and 8.8 with
+  // four, 2400 rows 18.6 and 19.2, 5000 rows 37.9 and 34.9, 14,700 rows 102 and 83)
+  const bool many = g->T > kSmCount * 4 * kAppendRows * 3 / 2;
   const unsigned grid = (unsigned)(many ? (g->T + kAppendRows - 1) / kAppendRows : g->T);
 #define ARCS_ROWS(TYPE, D)                                                                \
   do {                                                                                    \
