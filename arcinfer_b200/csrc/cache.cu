@@ -12,28 +12,29 @@ namespace arcs {
 // go stale, and the same pages go out whatever was given back in which order before.
 constexpr int kAllocThreads = 1024;
 
-__device__ __forceinline__ int block_scan_exclusive(int v, int* warp_sums, int* total) {
+// (in 64 bits: 4096 slots may ask for more pages than an int counts)
+__device__ __forceinline__ long long block_scan_exclusive(long long v, long long* warp_sums, long long* total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+  long long x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    const long long y = __shfl_up_sync(0xFFFFFFFFu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) warp_sums[w] = x;
   __syncthreads();
   if (w == 0) {
-    int y = warp_sums[lane];
+    long long y = warp_sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(0xFFFFFFFFu, y, o);
+      const long long z = __shfl_up_sync(0xFFFFFFFFu, y, o);
       if (lane >= o) y += z;
     }
     warp_sums[lane] = y;
   }
   __syncthreads();
   *total = warp_sums[31];
-  const int before = (w ? warp_sums[w - 1] : 0) + x - v;
+  const long long before = (w ? warp_sums[w - 1] : 0) + x - v;
   __syncthreads();
   return before;
 }
@@ -41,9 +42,9 @@ __device__ __forceinline__ int block_scan_exclusive(int v, int* warp_sums, int* 
 // `ask`: extra[] of reserve, parent[] of fork. done: fork's [slots], 1 where a copy was made.
 template <bool FORK>
 __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, const int32_t* __restrict__ ask, int32_t* __restrict__ done) {
-  __shared__ int pre[kMaxSlots + 1];   // pages that the slots before this one take
+  __shared__ int pre[kMaxSlots + 1];   // pages that the slots before this one take (at most INT_MAX: more than there are)
   __shared__ int base[kMaxSlots];      // where in the slot's list the first new page goes; -1: nothing is done for the slot
-  __shared__ int warp_sums[32];
+  __shared__ long long warp_sums[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (FORK) pdl_trigger();
 
@@ -97,14 +98,15 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
     }
     __syncthreads();
   }
-  int sum = 0;
+  long long asked = 0;
   for (int s0 = 0; s0 < c.slots; s0 += kAllocThreads) {
     const int s = s0 + tid;
-    int all;
-    const int before = block_scan_exclusive(s < c.slots ? pre[s] : 0, warp_sums, &all);
-    if (s < c.slots) pre[s] = sum + before;
-    sum += all;
+    long long all;
+    const long long before = block_scan_exclusive(s < c.slots ? pre[s] : 0, warp_sums, &all);
+    if (s < c.slots) pre[s] = (int)min(asked + before, 0x7FFFFFFFll);
+    asked += all;
   }
+  const int sum = (int)min(asked, 0x7FFFFFFFll);
   if (tid == 0) pre[c.slots] = sum;
   __syncthreads();
 
@@ -122,10 +124,10 @@ __global__ void __launch_bounds__(kAllocThreads) alloc_kernel(const CacheDev c, 
       b[j] = __ballot_sync(0xFFFFFFFFu, count[j] == 0);
       mine += __popc(b[j]);
     }
-    int all;
-    int r0 = found + block_scan_exclusive(lane == 0 ? mine : 0, warp_sums, &all);
+    long long all;
+    int r0 = found + (int)block_scan_exclusive(lane == 0 ? mine : 0, warp_sums, &all);
     r0 = __shfl_sync(0xFFFFFFFFu, r0, 0);
-    found += all;
+    found += (int)all;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int r = r0 + __popc(b[j] & ((1u << lane) - 1u));
@@ -573,11 +575,11 @@ extern "C" int arcs_cache_fork(const arcs_cache* cache, const int32_t* parent, i
   if (int inj = fault_injected()) return inj;
   if (const char* f = cache_fault(cache, true)) return bad_argument("cache_fork", f);
   if (!parent || !done) return bad_argument("cache_fork", "no list of parents, or none for what was done");
+  if ((int64_t)cache->layers * 2 * cache->heads > 65535) return bad_argument("cache_fork", "layers x heads of the cache is above 32767");
   const CacheDev c = cache_dev(cache);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   alloc_kernel<true><<<1, kAllocThreads, 0, st>>>(c, parent, done);
   if (int rc = check_launch("cache_fork")) return rc;
-  if ((int64_t)c.layers * 2 * c.heads > 65535) return bad_argument("cache_fork", "layers x heads is above 32767");
   const dim3 grid((unsigned)c.slots, (unsigned)(c.layers * 2 * c.heads));
   launch_behind(fork_copy_kernel, grid, dim3(256), 0, st, c, parent, done);
   return check_launch("cache_fork");
@@ -598,7 +600,7 @@ extern "C" int arcs_cache_compact(const arcs_cache* cache, const int32_t* kept, 
   const CacheDev c = cache_dev(cache);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t cols = (int64_t)c.layers * 2 * c.heads * (c.dim / 8);
-  if (cols > 0x7FFFFF00ll) return bad_argument("cache_compact", "layers x heads x dim is too large");
+  if (cols > 0x3FFFFFFFll) return bad_argument("cache_compact", "layers x heads x dim is too large");
   const int64_t most = (cols + 255) / 256, fill = (4 * kSmCount + c.slots - 1) / c.slots;
   compact_move_kernel<<<dim3((unsigned)(most < fill ? most : fill), (unsigned)c.slots), 256, 0, st>>>(c, kept, path, path_stride);
   if (int rc = check_launch("cache_compact")) return rc;

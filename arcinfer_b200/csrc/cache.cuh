@@ -30,7 +30,7 @@ inline const char* cache_fault(const arcs_cache* c, bool needs_ref) {
   if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return "the cache's page_size is not 16, 32, 64, 128 or 256";
   if (c->layers < 1 || c->n_pages < 1 || c->heads < 1 || c->heads > 1024 || c->max_pages < 1) return "a size of the cache is below 1, or heads above 1024";
   if (c->slots < 1 || c->slots > kMaxSlots) return "the cache's slots are not 1 .. 4096";
-  if ((int64_t)c->max_pages * c->page_size > 0x7FFFFF00ll) return "a slot of the cache could hold more than 2^31 tokens";
+  if ((int64_t)c->max_pages * c->page_size > 0x7FFF0000ll) return "a slot of the cache could hold more than 2^31 tokens";
   if (((c->layer_stride | c->page_stride | c->head_stride | c->token_stride) & 7) || c->layer_stride < 0 || c->page_stride < 0 ||
       c->head_stride < c->dim || c->token_stride < c->dim || (c->layers > 1 && c->layer_stride < c->dim) || (c->n_pages > 1 && c->page_stride < c->dim))
     return "a stride of the cache is not a multiple of 8 elements, or below dim";

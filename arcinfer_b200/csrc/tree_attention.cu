@@ -198,7 +198,9 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
   RowPlan r;
   if (plan_rows(c, &r)) {
     const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = 128, part = c->dim == 256 ? 64 : 128;  // (as in TilePlan)
-    if ((((int64_t)c->max_pages * c->page_size + keys - 1) / keys) * c->slots * c->heads * ((rows + most - 1) / most) > 0x0FFFFFFFll)
+    // (units of cost are counted in 31 bits: 6 a tile and 18 an item at most)
+    const int64_t tiles = ((int64_t)c->max_pages * c->page_size + keys - 1) / keys, items = (int64_t)c->slots * c->heads * ((rows + most - 1) / most);
+    if ((tiles * TilePlan<128, kPair>::kCost + TilePlan<128, kPair>::kItemCost) > 0x7FFFFFFFll / items)
       return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
     if (!encode_tiled()) return set_error(ARCS_ERR_CUDA, "tree_attention: the driver makes no tensor maps");
     CUtensorMap mk, mv;

@@ -19,7 +19,7 @@ struct TreeDev {
   // the tile kernel's
   int32_t by_row, page_rows, head_rows, no_row;  // where a page's rows lie in the tensor maps; a row behind the last
   int32_t part_rows;                             // rows of a block of partial results
-  uint32_t* prefix;                              // [slots + 1] units of work before a slot
+  uint32_t* prefix;                              // [slots + 2] units of work before a slot, and what an item counts for itself
   float2* part_stat;                             // [CTAs][2][part_rows] (maximum in log2, sum)
   float4* part;                                  // [CTAs][2][dim / 4][part_rows]: a warp's rows side by side where they are written
 };
@@ -289,7 +289,7 @@ __global__ void __maxnreg__(152)
   unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this piece and the next
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
   volatile int* fail = reinterpret_cast<volatile int*>(s_tmem + 1);
-  uint32_t* s_begin = s_tmem + 2;  // [3] first slot, units before it, units in all
+  uint32_t* s_begin = s_tmem + 2;  // [2] first slot, units before it
   uint32_t* s_sums = s_tmem + 5;   // [12]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
   pdl_trigger();

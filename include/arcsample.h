@@ -480,7 +480,9 @@ int arcs_cache_append(const arcs_append_args* args, void* stream);
  * 0 .. i. Query head h reads key head h / (Hq / heads). A row that sees nothing gets zeros and lse
  * -inf. What lies in masked places, and behind the last node, has no influence, NaN included.
  * Scores, statistics and sums are held in 32 bits; the weights are rounded to the cache's dtype before
- * the product with the values. A slot whose lists do not hold its tokens, or with more than max_nodes
+ * the product with the values. Pools whose page stride (and, unless a token's heads lie side by side, head
+ * stride) is a whole number of token strides take the tensor cores; others a plain kernel many times slower.
+ * `out` may be `q` itself (the same strides). A slot whose lists do not hold its tokens, or with more than max_nodes
  * nodes, raises ARCS_ERR_PAGE and its rows hold no result. */
 typedef struct {
   const arcs_cache* cache;     /* (host); `ref` is not used */

@@ -24,6 +24,9 @@ def pool(layers, n_pages, heads, page, dim, dtype, layout, fill=float("nan")):
         return torch.full((layers, n_pages, page, heads, dim), fill, dtype=dtype, device="cuda").transpose(2, 3)
     if layout == "pages":  # a page's layers side by side
         return torch.full((n_pages, layers, heads, page, dim), fill, dtype=dtype, device="cuda").transpose(0, 1)
+    if layout == "odd":  # pages that begin anywhere between two rows
+        n = heads * page * dim + 8
+        return torch.full((layers, n_pages * n), fill, dtype=dtype, device="cuda").as_strided((layers, n_pages, heads, page, dim), (n_pages * n, n, page * dim, dim, 1))
     # rows with a gap behind them, and pages with one
     wide = torch.full((layers, n_pages, heads * page + 3, dim + 8), fill, dtype=dtype, device="cuda")
     return wide[:, :, : heads * page, :dim].unflatten(2, (heads, page))

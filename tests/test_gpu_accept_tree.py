@@ -168,3 +168,62 @@ def test_a_whole_step(dim, dtype):
     ab.cache_free(tree, kv.i32([1] * (S + 1)))
     torch.cuda.synchronize()
     assert int(tree.ref.sum().item()) == 0
+
+
+def test_a_step_captured_and_replayed():
+    """reserve, append, attention, acceptance and compaction in one graph, replayed over a growing cache on a stream
+    of its own, against the same calls one by one"""
+    import arcinfer_b200 as ab
+    import kvutil as kv
+
+    S, N, heads, Hq, dim, layers = 5, 9, 2, 8, 128, 3
+    g = np.random.default_rng(9)
+    lens = [0, 17, 200, 16, 63]
+    off, parent, depth, mask = ab.tree_lists([kv.random_parents(g, N) for _ in range(S)])
+    T = int(off[-1])
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(9)
+    qkv = torch.randn(layers, T, Hq + 2 * heads, dim, generator=gen, device="cuda").to(torch.bfloat16)
+    token, draft = kv.i32(g.integers(0, 2, T)), kv.i32(g.integers(0, 2, T))
+    slot = torch.from_numpy(np.repeat(np.arange(S), N)).cuda()
+    off, parent, depth, mask = kv.i32(off), kv.i32(parent), kv.i32(depth), torch.from_numpy(mask).cuda()
+    inv = torch.from_numpy(1e4 ** (-np.arange(0, dim, 2) / dim)).cuda()
+    room = kv.i32([N] * S)
+
+    def step(cache):
+        ab.cache_reserve(cache, room)
+        pos = cache.length[slot] + depth
+        outs = []
+        for layer in range(layers):
+            q, k, v = qkv[layer].split([Hq, heads, heads], dim=1)
+            q = ab.cache_append(cache, q, k, v, off, pos, inv, layer=layer)
+            outs.append(ab.tree_attention(q, cache, off, N, mask=mask, layer=layer)["out"])
+        acc = ab.accept_tree(token, draft, parent, off, N)
+        ab.cache_compact(cache, acc["kept"], acc["path"])
+        return outs, acc
+
+    a, b = (kv.make_cache(3, lens, [0] * S, heads, 16, dim, layers=layers, spare=40, max_pages=24)[0] for _ in range(2))
+    fresh = [x.clone() for x in (b.k, b.v, b.table, b.used, b.ref, b.length)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(b)  # (before the capture, once)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs, acc = step(b)
+    torch.cuda.synchronize()
+    for x, y in zip((b.k, b.v, b.table, b.used, b.ref, b.length), fresh):
+        x.copy_(y)
+    for _ in range(4):
+        want, wacc = step(a)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(a.status.item()) == 0 and int(b.status.item()) == 0
+        for x, y in zip(outs + list(acc.values()), want + list(wacc.values())):
+            assert torch.equal(x, y)
+        for name in ("table", "used", "ref", "length"):
+            assert torch.equal(getattr(a, name), getattr(b, name)), name
+        for x, y in ((a.k, b.k), (a.v, b.v)):
+            assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+    assert a.length.tolist() != lens

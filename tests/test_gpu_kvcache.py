@@ -181,6 +181,21 @@ def test_pages_run_out(spare):
     plain.check(cache, 10)
 
 
+def test_more_pages_asked_for_than_an_int_counts():
+    import arcinfer_b200 as ab
+    import kvutil as kv
+
+    S, most, P = 200, 1 << 24, 50  # 200 x 2^24 pages
+    z = torch.zeros(1, P, 1, 16, 64, dtype=torch.bfloat16, device="cuda")
+    cache = ab.KVCache(z, z.clone(), torch.empty(S, most, dtype=torch.int32, device="cuda"), kv.i32(np.zeros(S)), kv.i32(np.zeros(P)), kv.i32(np.zeros(S)))
+    extra = np.full(S, 2**28)
+    extra[:2] = 20, 40
+    ab.cache_reserve(cache, kv.i32(extra))
+    torch.cuda.synchronize()
+    assert int(cache.status.item()) == 10 and cache.used.tolist() == [2, 3] + [0] * (S - 2)
+    assert cache.table[0, :2].tolist() == [0, 1] and cache.table[1, :3].tolist() == [2, 3, 4] and cache.ref.tolist() == [1] * 5 + [0] * 45
+
+
 def test_fork_refuses_and_runs_out():
     import arcinfer_b200 as ab
     import kvutil as kv

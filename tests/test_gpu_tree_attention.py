@@ -28,7 +28,7 @@ def _check(cache, rows, off, masks, q, got, lens, scale=None, layer=0):
     kv.check_attention(got["out"], got.get("lse"), q, rows, lens, off, masks, cache.dim**-0.5 if scale is None else scale, layer)
 
 
-@pytest.mark.parametrize("layout", ["heads", "tokens", "gap"])
+@pytest.mark.parametrize("layout", ["heads", "tokens", "gap", "odd"])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("dim,page,Hq,heads", [(64, 16, 8, 8), (64, 256, 8, 1), (128, 16, 14, 2), (128, 32, 2, 2), (128, 64, 32, 2), (128, 128, 10, 2), (256, 16, 4, 4), (256, 64, 16, 2)])
 def test_against_64_bits(dim, page, Hq, heads, dtype, layout):
@@ -69,6 +69,8 @@ def test_many_short_texts(dim, Hq, heads, most, dtype):
     for _ in range(3):
         got = ab.tree_attention(q, cache, kv.i32(off), most, mask=mask, want_lse=True)
         _check(cache, rows, off, masks, q, got, lens)
+    same = q.clone()  # results in place of the queries
+    assert torch.equal(ab.tree_attention(same, cache, kv.i32(off), most, mask=mask, out=same)["out"], got["out"])
 
 
 @pytest.mark.parametrize("slots", [129, 700])

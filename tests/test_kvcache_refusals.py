@@ -161,3 +161,27 @@ def test_tree_lists():
     for bad in ([-1, 1], [0], [-1, -1], [-1, 0, 5], [-1] + [0] * 64):
         with pytest.raises(ab.ArcsError):
             ab.tree_lists([bad])
+
+
+def test_calls_run_on_the_device_of_the_cache(monkeypatch):
+    """with another device current, the cache's is made current for the launch, and its stream is used"""
+    seen, current = [], [0]
+
+    class Device:
+        def __init__(self, dev):
+            self.index = dev.index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *a):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[-1], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    for index in (0, 1, 0):
+        kvc._enqueue(torch.device("cuda", index), lambda *a: seen.append((current[-1],) + a) or 0, "call", 5)
+    assert seen == [(0, 5, 100), (1, 5, 101), (0, 5, 100)] and current == [0]
+    with pytest.raises(ab.ArcsError, match="call"):
+        kvc._enqueue(torch.device("cuda", 1), lambda *a: 4, "call")
