@@ -26,6 +26,6 @@ def __getattr__(name):
 
         kvcache = importlib.import_module(".kvcache", __name__)
         value = kvcache if name == "kvcache" else getattr(kvcache, name)
-        globals()[name] = value  # (found without this function from now on: looking a name up so takes 5 us)
+        globals()[name] = value  # (found without this function from now on: looking a name up through it takes 1.6 us)
         return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
