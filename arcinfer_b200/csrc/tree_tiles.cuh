@@ -286,8 +286,8 @@ __global__ void __maxnreg__(152)
   uint64_t* bars = reinterpret_cast<uint64_t*>(handed + 128);
   uint64_t *full = bars, *empty = bars + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2, *ref_set = p_full + 2 /* [2][4] */, *q_first = ref_set + 8, *q_full = q_first + 1, *q_empty = q_full + 1,
            *item_done = q_empty + 1, *sums_done = item_done + 1, *stat_full = sums_done + 1, *sums_free = stat_full + 1, *drain = sums_free + 1;
-  unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [2] nodes whose values are not all finite, of this piece and the next
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 2);
+  unsigned long long* odd = reinterpret_cast<unsigned long long*>(drain + 1);  // [4] nodes whose values are not all finite: piece k's are in odd[k & 3]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(odd + 4);
   volatile int* fail = reinterpret_cast<volatile int*>(s_tmem + 1);
   uint32_t* s_begin = s_tmem + 2;  // [2] first slot, units before it
   uint32_t* s_sums = s_tmem + 5;   // [12]
@@ -314,8 +314,8 @@ __global__ void __maxnreg__(152)
         mbar_init(&s_full[i], 1);
         mbar_init(&p_half[i], 4);
         mbar_init(&p_full[i], 4);
-        odd[i] = 0;
       }
+      for (int i = 0; i < 4; ++i) odd[i] = 0;
       for (int i = 0; i < 8; ++i) mbar_init(&ref_set[i], 1);
       mbar_init(q_first, 8);
       mbar_init(q_full, 1);
@@ -747,7 +747,7 @@ __global__ void __maxnreg__(152)
             y = make_uint4(clean(y.x), clean(y.y), clean(y.z), clean(y.w));
             if (hit) {
               *v = y;
-              atomicOr(&odd[k & 1u], 1ull << (p0 + r - len));
+              atomicOr(&odd[k & 3u], 1ull << (p0 + r - len));
             }
           }
           fence_proxy_async();
@@ -785,7 +785,7 @@ __global__ void __maxnreg__(152)
         if (MODE != kSplit) f0 = 1.0f;  // (kShare: the sums are those of both groups)
         const uint64_t g0 = pair_of(f0 * inv, f0 * inv), g1 = pair_of(f1 * inv, f1 * inv);
         const int64_t block = (int64_t)cta * 2 + (p.t0 == 0);
-        const unsigned long long fix = odd[k & 1u] & bits;
+        const unsigned long long fix = odd[k & 3u] & bits;
         constexpr int kCols = MODE == kPair ? DIM : DIM / 2;
         const int c0 = MODE == kPair ? 0 : grp * kCols;
         if (live && (MODE == kPair || grp == 0)) {
@@ -863,7 +863,9 @@ __global__ void __maxnreg__(152)
           __syncwarp();
         }
       }
-      if (tid == 0) odd[(k + 1) & 1u] = 0;
+      // (the other warps may be at work on piece k + 1 by now and set its bits; none is in piece k + 2 before this warp, too,
+      // has arrived at the stat_full of k + 1, and none is still in piece k - 2)
+      if (tid == 0) odd[(k + 2) & 3u] = 0;
       tc_fence_before();
       arrive_warp(sums_free);
       rc0 += 2 * n * P::kSub;
