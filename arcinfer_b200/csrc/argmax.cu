@@ -262,8 +262,8 @@ extern "C" int arcs_accept_tree(const int32_t* token, const int32_t* draft, cons
                                 int32_t max_nodes, int32_t* accepted, int32_t* kept, int32_t* next, int32_t* path, int32_t path_stride, int32_t* status,
                                 void* stream) {
   if (int inj = fault_injected()) return inj;
-  if (!token || !draft || !parent || !node_off || !accepted || !kept || !next || !path || slots <= 0 || T < 0 || max_nodes < 1 || max_nodes > ARCS_TREE_MAX ||
-      path_stride < max_nodes)
+  if ((T > 0 && (!token || !draft || !parent)) || !node_off || !accepted || !kept || !next || !path || slots <= 0 || T < 0 || max_nodes < 1 ||
+      max_nodes > ARCS_TREE_MAX || path_stride < max_nodes)
     return set_error(ARCS_ERR_ARG, "accept_tree: bad argument");
   accept_tree_kernel<<<(unsigned)((slots + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(token, draft, parent, node_off, slots, T, max_nodes, accepted, kept,
                                                                                                  next, path, path_stride, status);

@@ -511,7 +511,8 @@ int arcs_tree_attention(const arcs_tree_attention_args* args, void* stream);
  * path (-1 for a slot without nodes), next[s] = the token chosen at its end (-1), path[s * path_stride
  * + i] = its nodes, the root first, then -1 up to max_nodes; kept[s] = nodes on it (accepted[s] + 1):
  * what arcs_cache_compact takes. A slot with more than max_nodes nodes, or rows outside 0 .. T - 1, is
- * taken as one without, and raises ARCS_ERR_PAGE in `status` (optional). */
+ * taken as one without, and raises ARCS_ERR_PAGE in `status` (optional). With T = 0 (a step in which no
+ * slot has nodes) token, draft and parent may be NULL. */
 int arcs_accept_tree(const int32_t* token, const int32_t* draft, const int32_t* parent, const int32_t* node_off, int32_t slots, int32_t T,
                      int32_t max_nodes, int32_t* accepted, int32_t* kept, int32_t* next, int32_t* path, int32_t path_stride, int32_t* status,
                      void* stream);
