@@ -110,6 +110,14 @@ bool make_map(CUtensorMap* map, const arcs_cache* c, const void* base, const Row
 
 int mode_of(int dim, int rows) { return dim == 256 ? kShare : rows > 128 ? kPair : kSplit; }
 int rows_of(int mode) { return mode == kPair ? 256 : 128; }
+// Units of cost that the tile kernel may have to count (in 31 bits, on the device): every slot as long as its list of pages.
+// Below 2^63: 2^12 slots x 2^10 heads x 2^5 blocks x (2^24 tiles x 6 + 18).
+int64_t most_units(const arcs_cache* c, int rows, int mode) {
+  const bool pair = mode == kPair;
+  const int64_t tiles = ((int64_t)c->max_pages * c->page_size + TilePlan<128, kPair>::kKeys - 1) / TilePlan<128, kPair>::kKeys;
+  const int64_t items = (int64_t)c->slots * c->heads * ((rows + rows_of(mode) - 1) / rows_of(mode));
+  return items * (tiles * (pair ? TilePlan<128, kPair>::kCost : TilePlan<128, kSplit>::kCost) + (pair ? TilePlan<128, kPair>::kItemCost : TilePlan<128, kSplit>::kItemCost));
+}
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 template <typename K>
@@ -170,6 +178,10 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
       g->out_token_stride < c->dim || g->out_head_stride < c->dim)
     return bad_argument("tree_attention", "a stride is not a multiple of 8 elements, or below dim");
   if ((reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->out)) & 15) return bad_argument("tree_attention", "a tensor is not 16-byte aligned");
+  RowPlan r;
+  const bool tiled = plan_rows(c, &r);
+  const int rows = g->max_nodes * (g->Hq / c->heads), mode = mode_of(c->dim, rows), most = rows_of(mode);
+  if (tiled && most_units(c, rows, mode) > 0x7FFFFFFFll) return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
   if (!g->workspace || g->workspace_bytes < arcs_tree_attention_workspace_bytes(c->slots, c->heads, g->Hq, c->dim, g->max_nodes) ||
       (reinterpret_cast<uintptr_t>(g->workspace) & 15))
     return set_error(ARCS_ERR_WORKSPACE, "tree_attention: workspace too small, or not 16-byte aligned");
@@ -195,13 +207,8 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
   const int64_t all_rows = (int64_t)g->T * g->Hq;
   if (all_rows > 0x1FFFFFFF0ll) return bad_argument("tree_attention", "too many rows");
 
-  RowPlan r;
-  if (plan_rows(c, &r)) {
-    const int rows = g->max_nodes * a.group, mode = mode_of(c->dim, rows), most = rows_of(mode), keys = 128, part = c->dim == 256 ? 64 : 128;  // (as in TilePlan)
-    // (units of cost are counted in 31 bits: 6 a tile and 18 an item at most)
-    const int64_t tiles = ((int64_t)c->max_pages * c->page_size + keys - 1) / keys, items = (int64_t)c->slots * c->heads * ((rows + most - 1) / most);
-    if ((tiles * TilePlan<128, kPair>::kCost + TilePlan<128, kPair>::kItemCost) > 0x7FFFFFFFll / items)
-      return bad_argument("tree_attention", "slots x places x heads x nodes is too large");
+  if (tiled) {
+    const int keys = 128, part = c->dim == 256 ? 64 : 128;  // (as in TilePlan)
     if (!encode_tiled()) return set_error(ARCS_ERR_CUDA, "tree_attention: the driver makes no tensor maps");
     CUtensorMap mk, mv;
     if (!make_map(&mk, c, a.c.k, r, keys) || !make_map(&mv, c, a.c.v, r, part)) return set_error(ARCS_ERR_CUDA, "tree_attention: no tensor map for these pools");

@@ -482,6 +482,9 @@ int arcs_cache_append(const arcs_append_args* args, void* stream);
  * Scores, statistics and sums are held in 32 bits; the weights are rounded to the cache's dtype before
  * the product with the values. Pools whose page stride (and, unless a token's heads lie side by side, head
  * stride) is a whole number of token strides take the tensor cores; others a plain kernel many times slower.
+ * The former count their work in 31 bits, as if every slot were as long as its list of pages: with R = max_nodes x (Hq / heads)
+ * and tiles = max_pages x page_size / 128, rounded up, they want slots x heads x ceil(R / 128) x (tiles + 4) < 2^31, for R > 128
+ * at dim 64 and 128 slots x heads x ceil(R / 256) x (6 tiles + 18) < 2^31; ARCS_ERR_ARG beyond.
  * `out` may be `q` itself (the same strides). A slot whose lists do not hold its tokens, or with more than max_nodes
  * nodes, raises ARCS_ERR_PAGE and its rows hold no result. */
 typedef struct {
