@@ -171,7 +171,7 @@ extern "C" int arcs_tree_attention(const arcs_tree_attention_args* g, void* stre
   if (g->layer < 0 || g->layer >= c->layers) return bad_argument("tree_attention", "no such layer");
   if (g->T < 0 || g->Hq < 1 || g->Hq % c->heads || g->Hq / c->heads > 64) return bad_argument("tree_attention", "T or Hq out of range, or Hq not a multiple of the key heads");
   if (g->max_nodes < 1 || g->max_nodes > ARCS_TREE_MAX) return bad_argument("tree_attention", "max_nodes is not 1 .. 64");
-  if (!(g->scale > 0.0f) || g->scale > 3e38f) return bad_argument("tree_attention", "scale is not a positive number");
+  if (!(g->scale > 0.0f) || g->scale * 1.4426950408889634f > 3.4028235e38f) return bad_argument("tree_attention", "scale is not a positive number");
   if (g->T == 0) return ARCS_OK;
   if (!g->q || !g->out || !g->node_off) return bad_argument("tree_attention", "a null pointer");
   if (((g->q_token_stride | g->q_head_stride | g->out_token_stride | g->out_head_stride) & 7) || g->q_token_stride < c->dim || g->q_head_stride < c->dim ||

@@ -500,7 +500,7 @@ typedef struct {
   const uint64_t* mask;        /* [T] or NULL */
   int32_t max_nodes;           /* 1 .. ARCS_TREE_MAX: no slot has more (the step's largest tree, not the largest there may ever be: it
                                   decides how the rows are cut into tiles) */
-  float scale;                 /* > 0 */
+  float scale;                 /* > 0, and scale * log2 e finite */
   void* workspace;             /* arcs_tree_attention_workspace_bytes(), 16-byte aligned; needs no initialisation; one for each call that may overlap another */
   size_t workspace_bytes;
 } arcs_tree_attention_args;
