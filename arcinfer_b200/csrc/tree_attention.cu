@@ -4,7 +4,9 @@
 namespace arcs {
 
 // For pools whose rows no tensor map can name (strides that are not multiples of one another): one warp a
-// row, a running maximum and sum over the places it sees, the values added up as they come.
+// row, a running maximum and sum over the places it sees, the values added up as they come. What bounds it is one
+// trip to memory after the other for every place: one token over 4096 takes 2.6 ms (18 us on the tensor cores), 24
+// nodes of 16 heads of 256 over 131071 tokens 153 ms (88 us).
 template <typename T, int DIM>
 __global__ void __launch_bounds__(128) tree_rows_kernel(const TreeDev a) {
   constexpr int kPer = DIM / 32;
@@ -137,7 +139,7 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TreeDev& a,
   using P = TilePlan<DIM, MODE>;
   static std::atomic<unsigned long long> attr_done{0}, room_done{0};
   cudaError_t e = ensure_dynamic_smem(tree_tiles_kernel<T, DIM, MODE>, P::kSmem, attr_done);
-  // (all of the SM's memory to be shared memory, not as much as this kernel asks for: join_kernel's CTA is to fit beside)
+  // (all of the SM's memory to be shared memory, not as much as this kernel asks for: with kSplit, and at dim 64, join_kernel's CTA is to fit beside)
   if (e == cudaSuccess) e = ensure_carveout(tree_tiles_kernel<T, DIM, MODE>, room_done);
   if (e != cudaSuccess) return set_error(ARCS_ERR_CUDA, cudaGetErrorString(e));
   tree_tiles_kernel<T, DIM, MODE><<<kCtas, kTileThreads, P::kSmem, st>>>(mk, mv, a);

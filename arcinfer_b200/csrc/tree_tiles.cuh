@@ -694,6 +694,10 @@ __global__ void __maxnreg__(152)
           }
           const float ref = W::kShift - (m == -INFINITY ? 0.0f : m);
           const uint64_t ref2 = pair_of(ref, ref);
+          // The weights are rounded to 16 bits, once, because the product with the values takes both operands in one 16-bit
+          // type; their sum is taken before that. It costs half a step of each weight: bf16 results are off by 2.3e-3 of
+          // their length where the rounding of the result alone makes 1.7e-3, fp16 ones by 2.8e-4 and 2.1e-4. A second
+          // product with what was rounded off would take it away, and double the time of the products with the values.
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int i = 0; i < kKeys / 32; ++i) {
@@ -886,7 +890,9 @@ __global__ void __maxnreg__(152)
 // share a row's pieces (FEW: the four warps do, too). It asks for some pieces at a time, their statistics
 // beside them: what bounds it is the latency of one such round, 1.7 us for pieces that other SMs have just
 // written. Small enough
-// (56 registers, 128 threads) to be on the SM, its way found, while the last pieces are still worked on.
+// (56 registers, 128 threads) to be on the SM, its way found, while the last pieces are still worked on, where the
+// tiles leave it shared memory: with kSplit, and at dim 64 (195 KB of 228). With kPair at dim 128 and kShare the
+// tiles take all of it, and a CTA of this kernel begins when one of theirs has left.
 constexpr int kJoinThreads = 128;
 template <int DIM, bool FEW>
 struct JoinPlan {

@@ -479,9 +479,12 @@ int arcs_cache_append(const arcs_append_args* args, void* stream);
  * are ignored; a node's own bit is taken as it stands, too). mask NULL: a chain, node i sees the nodes
  * 0 .. i. Query head h reads key head h / (Hq / heads). A row that sees nothing gets zeros and lse
  * -inf. What lies in masked places, and behind the last node, has no influence, NaN included.
- * Scores, statistics and sums are held in 32 bits; the weights are rounded to the cache's dtype before
- * the product with the values. Pools whose page stride (and, unless a token's heads lie side by side, head
- * stride) is a whole number of token strides take the tensor cores; others a plain kernel many times slower.
+ * Scores, statistics and sums are held in 32 bits; on the tensor cores the weights are rounded to the cache's
+ * dtype before the product with the values, which costs half a step of rounding beside the result's own (the
+ * plain kernel holds them in 32 bits). A prompt goes through it in chains of ARCS_TREE_MAX nodes, each of which
+ * reads the text again. Pools whose page stride (and, unless a token's heads lie side by side, head
+ * stride) is a whole number of token strides take the tensor cores; others a plain kernel
+ * 140 times slower and more (2.6 ms for one token over 4096).
  * The former count their work in 31 bits, as if every slot were as long as its list of pages: with R = max_nodes x (Hq / heads)
  * and tiles = max_pages x page_size / 128, rounded up, they want slots x heads x ceil(R / 128) x (tiles + 4) < 2^31, for R > 128
  * at dim 64 and 128 slots x heads x ceil(R / 256) x (6 tiles + 18) < 2^31; ARCS_ERR_ARG beyond.
