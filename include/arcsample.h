@@ -479,6 +479,7 @@ int arcs_cache_append(const arcs_append_args* args, void* stream);
  * are ignored; a node's own bit is taken as it stands, too). mask NULL: a chain, node i sees the nodes
  * 0 .. i. Query head h reads key head h / (Hq / heads). A row that sees nothing gets zeros and lse
  * -inf. What lies in masked places, and behind the last node, has no influence, NaN included.
+ * An infinite value shows in the rows that see it: a node's as it stands, a settled token's as NaN where its weight rounds to nothing.
  * Scores, statistics and sums are held in 32 bits; on the tensor cores the weights are rounded to the cache's
  * dtype before the product with the values, which costs half a step of rounding beside the result's own (the
  * plain kernel holds them in 32 bits). A prompt goes through it in chains of ARCS_TREE_MAX nodes, each of which
